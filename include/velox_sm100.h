@@ -361,6 +361,103 @@ int velox_sm100_add_bf16(float* acc, const uint16_t* xb, long long len);
 /* f32 -> bf16 twin (RNE), as velox_bf16_bits (velox_common.cuh:74-82). */
 int velox_sm100_bf16_twin(const float* x, uint16_t* xb, long long len);
 
+/* ---- attention over a 4-bit key/value cache -----------------------------------------------------
+ *
+ * What stands between the q|k|v linears and the o linear: the step's plan, the norms and rotation of
+ * the heads with the write into the cache, and the attention that reads it. Counterparts in the
+ * reference: qk_norm_rope_kv and the quantised-KV store / attention launchers
+ * (crates/velox-cuda/kernels/portable.cu, portable_kv.cu); the storage format and the argument
+ * lists are this library's own.
+ *
+ * The cache holds K and V as NVFP4 (E2M1 codes, an E4M3 scale per 16 values along the head, one divisor
+ * for K and one for V: value = code * scale / divisor). `blocks` is [pages][kv_heads][page_size / 16]
+ * blocks of 18 * head_dim bytes, 16-byte aligned; a block is 16 tokens:
+ *   K codes   [16 tokens][head_dim/2], two codes per byte, the even dimension in the low nibble;
+ *   V codes   [2][8][4][2][head_dim/16]: at [p][g][t][j] token 8p + 2t + j, bytes g*head_dim/16 ..;
+ *   K scales  [8][4][2][head_dim/64]: at [r][t][h][i] token 8h + r, group t*head_dim/64 + i;
+ *   V scales  [head_dim/16][4][2][2]: at [group][t][p][j] token 8p + 2t + j.
+ * A scale byte is read as its low seven bits (0x7f: 480): every byte pattern is a finite number.
+ * head_dim 64 or 128, page_size 16, 32, 64 or 128, pages * page_size < 2^31. A slot is
+ * page * page_size + the token's offset in the page. Head dims, page sizes or head counts outside
+ * these return VELOX_ERR_UNSUPPORTED. Device-side values are bounds-checked in the kernels: a slot
+ * or table entry outside the cache, a length outside the table or a row outside the buffers is
+ * skipped as described at each call. */
+typedef struct velox_sm100_kv4_cache {
+    uint8_t* blocks;
+    int64_t pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    float k_divisor;
+    float v_divisor;
+    int32_t reserved;      /* 0 */
+} velox_sm100_kv4_cache;
+
+/* Page table, slot map and positions of one step, from the requests' lengths, on the device.
+ * Request b has cached[b] tokens in the cache and new_tokens[b] new ones (negative counts as 0). It has
+ * have = ceil(cached / page_size) pages in its row of table [requests, table_cols] and gets the pages it
+ * lacks, at most table_cols in all, from free_pages[*taken ..] in request order (an entry is -1 once
+ * n_free are used up). Outputs: table (the new entries only); cu [requests + 1], running sums of
+ * new_tokens; kv_lens [requests], cached + new_tokens as far as there are pages; per row t <
+ * min(tokens, cu[requests]) its position and its slot (-1 where its page is missing), -1 for both in the
+ * rows behind; *taken_out, pages used so far (may be `taken` itself); *status: 1 pages ran out, 2 a row of
+ * the table is full, 4 more new tokens than rows, added up; 0 if all is well. `ticket`: one word that is 0
+ * before the call and after it; calls that may run at the same time need one each. */
+int velox_sm100_kv4_plan(const int32_t* cached, const int32_t* new_tokens, int requests, int32_t* table,
+                         int table_cols, const int32_t* free_pages, int n_free, const int32_t* taken,
+                         int32_t* taken_out, int page_size, int tokens, int32_t* cu, int32_t* kv_lens,
+                         int32_t* positions, int32_t* slots, int32_t* status, uint32_t* ticket);
+
+/* Per head of q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]:
+ *   y = x / sqrt(mean(x^2) + eps) * (offset + weight)        (weight NULL: y = x)
+ *   the first `rot` dimensions rotated by the angles of the row's position (rope NULL: not):
+ *   pairs (i, i + rot/2), or (2i, 2i + 1) with `interleaved`: (a cos - b sin, b cos + a sin)
+ * in f32, rounded once to the output's type. rope is [rope_len, rot] f32: rot/2 cosines, then rot/2 sines per
+ * position; rot a multiple of 16, at most head_dim. Rows whose position is outside [0, rope_len) (any
+ * negative one without a rope; positions may be NULL then) are left as they were. in_f32 / out_f32: element
+ * types (1 f32, 0 bf16). Strides between tokens are in elements, heads are head_dim apart; pointers and
+ * strides keep 16-byte alignment. An output may be its own input. */
+int velox_sm100_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride, int in_f32,
+                             const float* q_weight, const float* k_weight, const float* rope, int rope_len, int rot,
+                             int interleaved, const int32_t* positions, void* q_out, long long q_out_stride,
+                             void* k_out, long long k_out_stride, int out_f32, int tokens, int heads, int kv_heads,
+                             int head_dim, float eps, int offset);
+
+/* The same pass with k and v [tokens, kv_heads, head_dim] written into the cache at slots[token] (a slot
+ * outside the cache: not written; no two rows of a call may share one). k is normed and rotated in
+ * f64 and rounded once to f32 before it is quantised, so its codes do not depend on the order of a
+ * sum. Quantisation is that of velox_sm100_quantize_act_nvfp4 with the cache's divisors. heads = 0 (q and
+ * q_out NULL): k and v only; with weights and rope NULL too this is the plain store. */
+int velox_sm100_qk_norm_rope_kv4(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                                 long long v_stride, int in_f32, const float* q_weight, const float* k_weight,
+                                 const float* rope, int rope_len, int rot, int interleaved, const int32_t* positions,
+                                 const int32_t* slots, const velox_sm100_kv4_cache* cache, void* q_out,
+                                 long long q_out_stride, int out_f32, int tokens, int heads, float eps, int offset);
+
+/* Exact decode of the rows at slots[0 .. tokens) to k_out / v_out [tokens, kv_heads, head_dim] (either may be
+ * NULL), f32 or bf16: code * scale / divisor, rounded once. Rows whose slot is outside the cache are left
+ * as they were. */
+int velox_sm100_kv4_rows(const velox_sm100_kv4_cache* cache, const int32_t* slots, int tokens, void* k_out,
+                         void* v_out, int out_f32);
+
+/* out[row] = sum_j softmax_j(scale * q[row] . k_j) v_j over the cached tokens of the row's request.
+ * Rows cu[b] .. cu[b + 1] of q and out [tokens, heads, head_dim] bf16 are the last tokens of request b, whose
+ * kv_lens[b] tokens lie in the pages of its table row; row i of n stands at position kv_len - n + i and sees
+ * j < kv_len, j <= position if `causal`, j > position - window if window > 0. Query head h reads kv head
+ * h / (heads / kv_heads). A row that sees nothing gets zeros; rows outside every request are left as they
+ * were; tokens of a page outside the cache are not seen. max_new: at least the largest number of new rows of
+ * any request (requests with more are left out), which selects the kernels. Sums and softmax are f32; q is
+ * taken to f16 after scaling each row by a power of two, probabilities are rounded to f16.
+ * workspace: velox_sm100_kv4_attention_workspace bytes (-1 where the shape is not served), 256-byte aligned,
+ * zero before its first use. The calls of one stream may share it; calls that may run at the same time, or
+ * captured graphs that are replayed at the same time, need one each. */
+long long velox_sm100_kv4_attention_workspace(int heads, int kv_heads, int head_dim);
+int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* out, long long out_stride,
+                              const velox_sm100_kv4_cache* cache, const int32_t* table, int table_cols,
+                              const int32_t* cu, const int32_t* kv_lens, int requests, int tokens, int heads,
+                              float scale, int causal, int window, int max_new, void* workspace,
+                              long long workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,9 @@ def __getattr__(name):
     if name in ("Artifact", "ArtifactError", "Loader", "write_container"):
         from . import artifact
         return getattr(artifact, name)
+    if name in ("Kv4Cache", "Kv4Step", "rope_table"):
+        from . import kv4
+        return getattr(kv4, name)
     if name in ("LinearStack", "StackSpec"):
         from . import stack
         return getattr(stack, name)

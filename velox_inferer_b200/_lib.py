@@ -50,6 +50,13 @@ class Part(C.Structure):
     _fields_ = [("view", View), ("y", C.c_void_p), ("ld", C.c_int64), ("col", C.c_int64)]
 
 
+class Kv4CacheStruct(C.Structure):
+    """``velox_sm100_kv4_cache`` (include/velox_sm100.h)."""
+
+    _fields_ = [("blocks", C.c_void_p), ("pages", C.c_int64), ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("k_divisor", C.c_float), ("v_divisor", C.c_float), ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/velox_sm100.h declares
 _VP, _I, _LL, _F = C.c_void_p, C.c_int, C.c_longlong, C.c_float
 _PV = C.POINTER(View)
@@ -100,6 +107,14 @@ SIGNATURES = {
     "velox_sm100_add": (_I, [_VP, _VP, _LL]),
     "velox_sm100_add_rms_norm_twin": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _F, _I]),
     "velox_sm100_bf16_twin": (_I, [_VP, _VP, _LL]),
+    "velox_sm100_kv4_plan": (_I, [_VP, _VP, _I, _VP, _I, _VP, _I, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "velox_sm100_qk_norm_rope": (_I, [_VP, _LL, _VP, _LL, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _VP, _LL, _VP, _LL, _I, _I, _I,
+                                      _I, _I, _F, _I]),
+    "velox_sm100_qk_norm_rope_kv4": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _I, _VP, _VP, _VP, _I, _I, _I, _VP, _VP, _VP, _VP,
+                                          _LL, _I, _I, _I, _F, _I]),
+    "velox_sm100_kv4_rows": (_I, [_VP, _VP, _I, _VP, _VP, _I]),
+    "velox_sm100_kv4_attention_workspace": (C.c_longlong, [_I, _I, _I]),
+    "velox_sm100_kv4_attention": (_I, [_VP, _LL, _VP, _LL, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _F, _I, _I, _I, _VP, _LL]),
 }
 
 

@@ -10,6 +10,7 @@
 #include "common.cuh"
 #include "gemm.cuh"
 #include "kernels.cuh"
+#include "kv4.cuh"
 
 namespace vx {
 
@@ -696,5 +697,176 @@ int velox_sm100_add_bf16(float* acc, const uint16_t* xb, long long len) {
 }
 
 int velox_sm100_bf16_twin(const float* x, uint16_t* xb, long long len) { return bf16_twin(x, xb, len); }
+
+// ---- 4-bit key/value cache -------------------------------------------------------------------------
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static int kv4_geom(const velox_sm100_kv4_cache* c, Kv4Geom& g) {
+    if (!c || !c->blocks || c->pages <= 0 || c->kv_heads <= 0) return VELOX_ERR_SHAPE;
+    if (!(c->k_divisor > 0.0f) || !(c->v_divisor > 0.0f)) return VELOX_ERR_SHAPE;
+    if (c->head_dim != 64 && c->head_dim != 128) return VELOX_ERR_UNSUPPORTED;
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return VELOX_ERR_UNSUPPORTED;
+    if (c->pages >= 0x80000000LL / c->page_size || c->kv_heads > 65535) return VELOX_ERR_UNSUPPORTED;
+    if (!aligned16(c->blocks)) return VELOX_ERR_UNSUPPORTED;
+    g.blocks = c->blocks;
+    g.pages = c->pages;
+    g.page_size = c->page_size;
+    g.kv_heads = c->kv_heads;
+    g.head_dim = c->head_dim;
+    g.k_div = c->k_divisor;
+    g.v_div = c->v_divisor;
+    return 0;
+}
+
+int velox_sm100_kv4_plan(const int32_t* cached, const int32_t* new_tokens, int requests, int32_t* table,
+                         int table_cols, const int32_t* free_pages, int n_free, const int32_t* taken,
+                         int32_t* taken_out, int page_size, int tokens, int32_t* cu, int32_t* kv_lens,
+                         int32_t* positions, int32_t* slots, int32_t* status, uint32_t* ticket) {
+    if (requests < 0 || tokens < 0 || table_cols < 0 || n_free < 0) return VELOX_ERR_SHAPE;
+    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return VELOX_ERR_UNSUPPORTED;
+    if (!taken || !taken_out || !cu || !status || !ticket) return VELOX_ERR_SHAPE;
+    if (requests > 0 && (!cached || !new_tokens || !kv_lens || (table_cols > 0 && !table))) return VELOX_ERR_SHAPE;
+    if ((tokens > 0 && (!positions || !slots)) || (n_free > 0 && !free_pages)) return VELOX_ERR_SHAPE;
+    return kv4_plan(cached, new_tokens, requests, table, table_cols, free_pages, n_free, taken, taken_out, page_size, tokens,
+                    cu, kv_lens, positions, slots, status, ticket);
+}
+
+// Strides and pointers of one [tokens, heads, head_dim] operand (elements of `size` bytes).
+static int check_rows(const void* p, long long stride, int heads, int head_dim, int size) {
+    if (!p || stride < (long long)heads * head_dim) return VELOX_ERR_SHAPE;
+    if (!aligned16(p) || stride * size % 16 != 0) return VELOX_ERR_UNSUPPORTED;
+    return 0;
+}
+
+static int check_rope(const Kv4RopeArgs& a) {
+    if (a.tokens < 0 || a.heads < 0 || a.kv_heads < 0 || !(a.eps >= 0.0f)) return VELOX_ERR_SHAPE;
+    if (a.head_dim != 64 && a.head_dim != 128) return VELOX_ERR_UNSUPPORTED;
+    if (a.heads > 65535 || a.kv_heads > 65535) return VELOX_ERR_UNSUPPORTED;
+    if (!aligned16(a.q_weight) || !aligned16(a.k_weight) || !aligned16(a.rope)) return VELOX_ERR_UNSUPPORTED;
+    if (a.rope) {
+        if (!a.positions || a.rope_len <= 0 || a.rot <= 0 || a.rot > a.head_dim) return VELOX_ERR_SHAPE;
+        if (a.rot % 16 != 0) return VELOX_ERR_UNSUPPORTED;
+    }
+    return 0;
+}
+
+int velox_sm100_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride, int in_f32,
+                             const float* q_weight, const float* k_weight, const float* rope, int rope_len, int rot,
+                             int interleaved, const int32_t* positions, void* q_out, long long q_out_stride,
+                             void* k_out, long long k_out_stride, int out_f32, int tokens, int heads, int kv_heads,
+                             int head_dim, float eps, int offset) {
+    Kv4RopeArgs a{};
+    a.q = q; a.k = k;
+    a.q_stride = q_stride; a.k_stride = k_stride;
+    a.in_f32 = in_f32 != 0; a.out_f32 = out_f32 != 0;
+    a.q_weight = q_weight; a.k_weight = k_weight;
+    a.rope = rope; a.rope_len = rope_len; a.rot = rot; a.interleaved = interleaved != 0;
+    a.positions = positions;
+    a.q_out = q_out; a.k_out = k_out;
+    a.q_out_stride = q_out_stride; a.k_out_stride = k_out_stride;
+    a.tokens = tokens; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim;
+    a.eps = eps; a.offset = offset != 0;
+    int rc = check_rope(a);
+    if (rc != 0) return rc;
+    if (heads + kv_heads <= 0) return VELOX_ERR_SHAPE;
+    const int in = a.in_f32 ? 4 : 2, out = a.out_f32 ? 4 : 2;
+    if (heads > 0) {
+        if ((rc = check_rows(q, q_stride, heads, head_dim, in)) != 0) return rc;
+        if ((rc = check_rows(q_out, q_out_stride, heads, head_dim, out)) != 0) return rc;
+    }
+    if (kv_heads > 0) {
+        if ((rc = check_rows(k, k_stride, kv_heads, head_dim, in)) != 0) return rc;
+        if ((rc = check_rows(k_out, k_out_stride, kv_heads, head_dim, out)) != 0) return rc;
+    }
+    if (tokens == 0) return 0;
+    return kv4_norm_rope(a);
+}
+
+int velox_sm100_qk_norm_rope_kv4(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                                 long long v_stride, int in_f32, const float* q_weight, const float* k_weight,
+                                 const float* rope, int rope_len, int rot, int interleaved, const int32_t* positions,
+                                 const int32_t* slots, const velox_sm100_kv4_cache* cache, void* q_out,
+                                 long long q_out_stride, int out_f32, int tokens, int heads, float eps, int offset) {
+    Kv4RopeArgs a{};
+    int rc = kv4_geom(cache, a.cache);
+    if (rc != 0) return rc;
+    a.q = q; a.k = k; a.v = v;
+    a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.in_f32 = in_f32 != 0; a.out_f32 = out_f32 != 0;
+    a.q_weight = q_weight; a.k_weight = k_weight;
+    a.rope = rope; a.rope_len = rope_len; a.rot = rot; a.interleaved = interleaved != 0;
+    a.positions = positions; a.slots = slots;
+    a.q_out = q_out; a.q_out_stride = q_out_stride;
+    a.tokens = tokens; a.heads = heads; a.kv_heads = cache->kv_heads; a.head_dim = cache->head_dim;
+    a.eps = eps; a.offset = offset != 0;
+    a.store = 1;
+    rc = check_rope(a);
+    if (rc != 0) return rc;
+    const int in = a.in_f32 ? 4 : 2, out = a.out_f32 ? 4 : 2;
+    if (heads > 0) {
+        if ((rc = check_rows(q, q_stride, heads, a.head_dim, in)) != 0) return rc;
+        if ((rc = check_rows(q_out, q_out_stride, heads, a.head_dim, out)) != 0) return rc;
+    }
+    if ((rc = check_rows(k, k_stride, a.kv_heads, a.head_dim, in)) != 0) return rc;
+    if ((rc = check_rows(v, v_stride, a.kv_heads, a.head_dim, in)) != 0) return rc;
+    if (tokens == 0) return 0;
+    if (!slots) return VELOX_ERR_SHAPE;
+    return kv4_norm_rope(a);
+}
+
+int velox_sm100_kv4_rows(const velox_sm100_kv4_cache* cache, const int32_t* slots, int tokens, void* k_out,
+                         void* v_out, int out_f32) {
+    Kv4Geom g{};
+    const int rc = kv4_geom(cache, g);
+    if (rc != 0) return rc;
+    if (tokens < 0 || (!k_out && !v_out)) return VELOX_ERR_SHAPE;
+    if (!aligned16(k_out) || !aligned16(v_out)) return VELOX_ERR_UNSUPPORTED;
+    if (tokens == 0) return 0;
+    if (!slots) return VELOX_ERR_SHAPE;
+    return kv4_rows(g, slots, tokens, k_out, v_out, out_f32 != 0);
+}
+
+static int check_heads(int heads, int kv_heads, int head_dim) {
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return VELOX_ERR_SHAPE;
+    if (head_dim != 64 && head_dim != 128) return VELOX_ERR_UNSUPPORTED;
+    if (heads > 65535) return VELOX_ERR_UNSUPPORTED;
+    return 0;
+}
+
+long long velox_sm100_kv4_attention_workspace(int heads, int kv_heads, int head_dim) {
+    if (check_heads(heads, kv_heads, head_dim) != 0) return -1;
+    return kv4_attention_workspace(heads, kv_heads, head_dim);
+}
+
+int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* out, long long out_stride,
+                              const velox_sm100_kv4_cache* cache, const int32_t* table, int table_cols,
+                              const int32_t* cu, const int32_t* kv_lens, int requests, int tokens, int heads,
+                              float scale, int causal, int window, int max_new, void* workspace,
+                              long long workspace_bytes) {
+    Kv4AttnArgs a{};
+    int rc = kv4_geom(cache, a.cache);
+    if (rc != 0) return rc;
+    rc = check_heads(heads, cache->kv_heads, cache->head_dim);
+    if (rc != 0) return rc;
+    if (requests < 0 || tokens < 0 || table_cols < 0 || window < 0 || max_new < 0) return VELOX_ERR_SHAPE;
+    if (!(scale > 0.0f) || scale > 1e30f) return VELOX_ERR_SHAPE;
+    if (requests == 0 || tokens == 0 || max_new == 0) return 0;
+    if ((rc = check_rows(q, q_stride, heads, cache->head_dim, 2)) != 0) return rc;
+    if ((rc = check_rows(out, out_stride, heads, cache->head_dim, 2)) != 0) return rc;
+    if (!cu || !kv_lens || (table_cols > 0 && !table)) return VELOX_ERR_SHAPE;
+    if (!workspace || workspace_bytes < kv4_attention_workspace(heads, cache->kv_heads, cache->head_dim)) return VELOX_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255) return VELOX_ERR_UNSUPPORTED;
+    a.q = q; a.q_stride = q_stride;
+    a.out = out; a.out_stride = out_stride;
+    a.table = table; a.cols = table_cols;
+    a.cu = cu; a.kv_lens = kv_lens;
+    a.requests = requests; a.tokens = tokens; a.heads = heads;
+    a.scale = scale; a.causal = causal != 0; a.window = window;
+    a.max_new = max_new < tokens ? max_new : tokens;
+    a.ws = reinterpret_cast<uint8_t*>(workspace);
+    a.ws_bytes = workspace_bytes;
+    return kv4_attention(a);
+}
 
 }  // extern "C"
