@@ -90,7 +90,8 @@ int velox_sm100_abi_version(void);
 
 /* Debug aid with no counterpart in the reference: synchronises the device and returns the status
  * word of the kernels that wait on something: 0, or the code of the first bounded wait that gave up
- * (1-5: an mbarrier inside a tensor-core kernel; 6: a peer's flag in a tensor-parallel step). The
+ * (1-5: an mbarrier inside a tensor-core kernel; 6: a peer's flag in a tensor-parallel step; 7: an mbarrier
+ * of the prefill attention over the 4-bit cache). The
  * kernel then went on without what it waited for and its output is meaningless. The word is sticky
  * until velox_sm100_debug_status_reset. Never call either on a hot path. */
 int velox_sm100_debug_status(void);

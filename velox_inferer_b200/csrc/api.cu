@@ -359,7 +359,9 @@ int velox_sm100_debug_status(void) {
     const int b = gemv_status_sync();
     if (b != 0) return b;
     const int c = gemv_tc_status_sync();
-    return c != 0 ? c : tp_status_sync();
+    if (c != 0) return c;
+    const int d = tp_status_sync();
+    return d != 0 ? d : kv4_status_sync();
 }
 
 int velox_sm100_debug_status_reset(void) {
@@ -369,6 +371,7 @@ int velox_sm100_debug_status_reset(void) {
     if (rc == 0) rc = gemv_status_reset();
     if (rc == 0) rc = gemv_tc_status_reset();
     if (rc == 0) rc = tp_status_reset();
+    if (rc == 0) rc = kv4_status_reset();
     return rc;
 }
 
@@ -836,7 +839,7 @@ static int check_heads(int heads, int kv_heads, int head_dim) {
 
 long long velox_sm100_kv4_attention_workspace(int heads, int kv_heads, int head_dim) {
     if (check_heads(heads, kv_heads, head_dim) != 0) return -1;
-    return kv4_attention_workspace(heads, kv_heads, head_dim);
+    return kv4_attention_workspace(head_dim);
 }
 
 int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* out, long long out_stride,
@@ -855,7 +858,7 @@ int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* o
     if ((rc = check_rows(q, q_stride, heads, cache->head_dim, 2)) != 0) return rc;
     if ((rc = check_rows(out, out_stride, heads, cache->head_dim, 2)) != 0) return rc;
     if (!cu || !kv_lens || (table_cols > 0 && !table)) return VELOX_ERR_SHAPE;
-    if (!workspace || workspace_bytes < kv4_attention_workspace(heads, cache->kv_heads, cache->head_dim)) return VELOX_ERR_SHAPE;
+    if (!workspace || workspace_bytes < kv4_attention_workspace(cache->head_dim)) return VELOX_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return VELOX_ERR_UNSUPPORTED;
     a.q = q; a.q_stride = q_stride;
     a.out = out; a.out_stride = out_stride;
@@ -865,7 +868,6 @@ int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* o
     a.scale = scale; a.causal = causal != 0; a.window = window;
     a.max_new = max_new < tokens ? max_new : tokens;
     a.ws = reinterpret_cast<uint8_t*>(workspace);
-    a.ws_bytes = workspace_bytes;
     return kv4_attention(a);
 }
 

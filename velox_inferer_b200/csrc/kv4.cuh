@@ -93,9 +93,17 @@ struct Kv4AttnArgs {
     int causal, window;
     int max_new;
     uint8_t* ws;
-    long long ws_bytes;
+    // set by the dispatcher: requests a kernel takes, by query rows per kv head: (min_rows, max_rows]; and where the
+    // parts of the decode kernel's split items lie in the workspace (its tickets are at the start)
+    int min_rows, max_rows;
+    long long decode_parts, prefill_tickets, prefill_parts;
 };
-long long kv4_attention_workspace(int heads, int kv_heads, int head_dim);
-int kv4_attention(const Kv4AttnArgs& a);
+long long kv4_attention_workspace(int head_dim);
+int kv4_attention(Kv4AttnArgs a);
+// many query rows per request, on the tcgen05 tensor cores
+int kv4_prefill(const Kv4AttnArgs& a, int blocks);
+long long kv4_prefill_parts_bytes(int blocks, int head_dim);
+int kv4_status_sync();
+int kv4_status_reset();
 
 }  // namespace vx

@@ -23,51 +23,10 @@
 // blocks to arrive joins them in token order: results do not depend on the order of arrival.
 #include "common.cuh"
 #include "kv4.cuh"
+#include "kv4_items.cuh"
 
 namespace vx {
 
-__device__ __forceinline__ uint4 ldg_stream16(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const uint8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t ldg_stream4(const uint8_t* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t ldg_stream2(const uint8_t* p) {
-    uint16_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
-    return v;
-}
-
-// Eight E2M1 codes of a word -> four f16x2 (byte b holds codes 2b, 2b + 1; the first in the low half).
-__device__ __forceinline__ void codes_to_f16(uint32_t word, uint32_t (&h)[4]) {
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-        : "r"(word));
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-// Scale bytes (as seven magnitude bits) to f16, times 2^-8, exactly: the E4M3 pattern moved up seven
-// places is the same number with f16's bias.
-__device__ __forceinline__ uint32_t scale_pair(uint32_t word, uint32_t sel) {   // sel: the two bytes, 0x4x4y
-    return (__byte_perm(word, 0, sel) << 7) & 0x3f803f80u;
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -80,18 +39,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-constexpr float NEG_BIG = -1e30f;   // "no score yet": finite, so that differences of it are numbers
-
 template <int D, int NT, int WARPS>
 struct DecodeCfg {
     static constexpr int ROWS = 8 * NT;            // query rows of an item
@@ -103,97 +50,6 @@ struct DecodeCfg {
     // a parked part: max, sum per row, then O
     static constexpr int PART = ROWS * (D + 2);
 };
-
-// What a request asks of this kernel.
-struct Request {
-    int row0, n, kv_len, row_tiles;
-    long long units;   // of one kv head
-};
-
-struct RowRange {
-    int lo, hi;   // tokens any of the rows sees
-};
-
-template <int ROWS>
-__device__ __forceinline__ RowRange rows_range(const Kv4AttnArgs& a, int G, const Request& r, int tile) {
-    const int first = r.kv_len - r.n + tile * ROWS / G;
-    const int last = r.kv_len - r.n + (min((tile + 1) * ROWS, r.n * G) - 1) / G;
-    RowRange x;
-    x.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-    x.hi = a.causal ? min(r.kv_len, last + 1) : r.kv_len;
-    return x;
-}
-
-template <int ROWS, int TILE>
-__device__ __forceinline__ int tiles_of(const RowRange& x) {
-    // an item that sees nothing still has one tile: its rows get zeros
-    return x.hi <= x.lo ? 1 : (x.hi + TILE - 1) / TILE - x.lo / TILE;
-}
-
-template <int ROWS, int TILE>
-__device__ __forceinline__ Request request_of(const Kv4AttnArgs& a, int G, int b) {
-    Request r;
-    r.row0 = min(max(a.cu[b], 0), a.tokens);
-    r.n = max(0, min(max(a.cu[b + 1], 0), a.tokens) - r.row0);
-    r.kv_len = (int)min((long long)max(a.kv_lens[b], 0), (long long)a.cols * a.cache.page_size);
-    if (r.n > a.max_new) r.n = 0;   // past the caller's hint: left out
-    r.row_tiles = (r.n * G + ROWS - 1) / ROWS;
-    r.units = 0;
-    for (int t = 0; t < r.row_tiles; t++) r.units += tiles_of<ROWS, TILE>(rows_range<ROWS>(a, G, r, t));
-    return r;
-}
-
-template <int D>
-struct KRegs {
-    uint32_t c[2][D / 32];   // two token rows of D/4 codes each
-    uint32_t s;
-};
-template <int D>
-struct VRegs {
-    uint32_t c[2][D / 32];   // [p]: tokens 8p + 2t, 8p + 2t + 1
-    uint32_t s;
-};
-
-template <int D>
-__device__ __forceinline__ void load_k(KRegs<D>& r, const uint8_t* blk, int lane) {
-    if (blk == nullptr) {
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) r.c[0][i] = r.c[1][i] = 0;
-        r.s = 0;
-        return;
-    }
-    if (D == 128) {
-        const uint4 x = ldg_stream16(blk + lane * 16), y = ldg_stream16(blk + 512 + lane * 16);
-        r.c[0][0] = x.x; r.c[0][1] = x.y; r.c[0][D / 32 - 2] = x.z; r.c[0][D / 32 - 1] = x.w;
-        r.c[1][0] = y.x; r.c[1][1] = y.y; r.c[1][D / 32 - 2] = y.z; r.c[1][D / 32 - 1] = y.w;
-        r.s = ldg_stream4(blk + 16 * D + lane * 4);
-    } else {
-        const uint2 x = ldg_stream8(blk + lane * 8), y = ldg_stream8(blk + 256 + lane * 8);
-        r.c[0][0] = x.x; r.c[0][1] = x.y;
-        r.c[1][0] = y.x; r.c[1][1] = y.y;
-        r.s = ldg_stream2(blk + 16 * D + lane * 2);
-    }
-}
-template <int D>
-__device__ __forceinline__ void load_v(VRegs<D>& r, const uint8_t* blk, int lane) {
-    if (blk == nullptr) {
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) r.c[0][i] = r.c[1][i] = 0;
-        r.s = 0;
-        return;
-    }
-    if (D == 128) {
-        const uint4 x = ldg_stream16(blk + 8 * D + lane * 16), y = ldg_stream16(blk + 8 * D + 512 + lane * 16);
-        r.c[0][0] = x.x; r.c[0][1] = x.y; r.c[0][D / 32 - 2] = x.z; r.c[0][D / 32 - 1] = x.w;
-        r.c[1][0] = y.x; r.c[1][1] = y.y; r.c[1][D / 32 - 2] = y.z; r.c[1][D / 32 - 1] = y.w;
-        r.s = ldg_stream4(blk + 17 * D + lane * 4);
-    } else {
-        const uint2 x = ldg_stream8(blk + 8 * D + lane * 8), y = ldg_stream8(blk + 8 * D + 256 + lane * 8);
-        r.c[0][0] = x.x; r.c[0][1] = x.y;
-        r.c[1][0] = y.x; r.c[1][1] = y.y;
-        r.s = ldg_stream4(blk + 17 * D + ((lane >> 3) * 4 + (lane & 3)) * 4);   // group g / 2 of lane (g, t)
-    }
-}
 
 // S^T of one block of 16 tokens: c[n] rows g, g + 8 = tokens, columns 2t, 2t + 1 of row tile n.
 template <int D, int NT>
@@ -260,87 +116,25 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     extern __shared__ float smem[];
     float* s_o = smem;                                   // [WARPS][ROWS][STRIDE]
     float* s_m = smem + WARPS * ROWS * C::STRIDE;        // [WARPS][ROWS] max, then sum
-    __shared__ long long s_red[WARPS + 1];
-    __shared__ int s_find[4];
-    __shared__ long long s_first;
+    __shared__ long long s_red[WARPS], s_found[2];
+    __shared__ int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int hkv = a.cache.kv_heads, G = a.heads / hkv, P16 = a.cache.page_size >> 4;
     if (tid == 0) grid_launch_dependents();
     grid_dependency_wait();
 
-    // ---- this block's run of units ----
-    long long mine = 0;
-    for (int b = tid; b < a.requests; b += C::THREADS) mine += request_of<ROWS, TILE>(a, G, b).units * hkv;
-    {
-        long long x = mine;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (lane == 0) s_red[warp] = x;
-    }
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; i++) total += s_red[i];
-    const int W = (int)min((long long)gridDim.x, total);
+    const Run run = find_run<ROWS, TILE, C::THREADS>(a, G, s_red, s_found);
+    if ((int)blockIdx.x >= run.blocks) return;
     const int cta = blockIdx.x;
-    if (cta >= W) return;
-    const long long u_begin = total * cta / W, u_end = total * (cta + 1) / W;
-    {   // the request that holds u_begin
-        long long before = 0;
-        for (int base = 0; base < a.requests; base += C::THREADS) {
-            const int b = base + tid;
-            const long long v = b < a.requests ? request_of<ROWS, TILE>(a, G, b).units * hkv : 0;
-            long long x = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 31) s_red[warp] = x;
-            __syncthreads();
-            long long pre = before, sum = 0;
-#pragma unroll
-            for (int i = 0; i < WARPS; i++) {
-                pre += i < warp ? s_red[i] : 0;
-                sum += s_red[i];
-            }
-            const long long lo = pre + x - v;
-            if (u_begin >= lo && u_begin < lo + v) {
-                s_find[0] = b;
-                s_first = lo;
-            }
-            before += sum;
-            if (before > u_begin) break;
-        }
-        __syncthreads();
-    }
-
-    int b = s_find[0];
-    long long req_first = s_first;   // first unit of request b
-    Request r = request_of<ROWS, TILE>(a, G, b);
-    long long u = u_begin;
-    const float soft = a.scale * 1.4426950408889634f / a.cache.k_div * 256.0f;   // 2^8: scale_pair's 2^-8
+    const float soft = score_factor(a);
     uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws);
-    float* parts = reinterpret_cast<float*>(a.ws + ((gridDim.x * 4 + 255) & ~255));
+    float* parts = reinterpret_cast<float*>(a.ws + a.decode_parts);
 
-    while (u < u_end) {
-        while (u >= req_first + r.units * hkv) {   // (requests without rows have no units)
-            req_first += r.units * hkv;
-            r = request_of<ROWS, TILE>(a, G, ++b);
-        }
-        // the item that holds u
-        const int h = (int)((u - req_first) / r.units);
-        long long item_first = req_first + (long long)h * r.units;
-        int rt = 0;
-        RowRange range = rows_range<ROWS>(a, G, r, 0);
-        int nt = tiles_of<ROWS, TILE>(range);
-        while (u >= item_first + nt) {
-            item_first += nt;
-            range = rows_range<ROWS>(a, G, r, ++rt);
-            nt = tiles_of<ROWS, TILE>(range);
-        }
-        const int k0 = (int)(u - item_first), k1 = (int)min((long long)nt, u_end - item_first);
+    Items<ROWS, TILE> it(a, G, run);
+    for (; it.next(a, G); it.done()) {
+        const Request& r = it.r;
+        const RowRange range = it.range;
+        const int b = it.b, h = it.h, rt = it.rt, k0 = it.k0, k1 = it.k1;
         const int tile0 = range.lo / TILE;
         const int rows = min(ROWS, r.n * G - rt * ROWS);
         const int qbase = r.kv_len - r.n;
@@ -375,15 +169,14 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int i = 0; i < D / 4; i++) amax = fmaxf(amax, fabsf(x[i]));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // largest |q| of the row into [1, 2) (a row of zeros, or of numbers below 2^-100, as it is)
-            const int e = min(max((int)(__float_as_uint(amax) >> 23), 27), 227) - 127;
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            const int e = row_exponent(amax);
+            const float down = pow2(-e);
 #pragma unroll
             for (int j = 0; j < D / 16; j++) {
                 qf[n][j][0] = pack_f16(x[4 * j] * down, x[4 * j + 1] * down);
                 qf[n][j][1] = pack_f16(x[4 * j + 2] * down, x[4 * j + 3] * down);
             }
-            const float up = soft * __uint_as_float((uint32_t)(127 + e) << 23);
+            const float up = soft * pow2(e);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int col = n * 8 + 2 * t + c;
@@ -542,10 +335,8 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     *reinterpret_cast<float2*>(s_o + (warp * ROWS + n * 8 + 2 * t + y) * C::STRIDE + i * 16 + 2 * g) =
                         make_float2(o[n][i][y], o[n][i][y + 2]);
         __syncthreads();
-        const bool whole = k0 == 0 && k1 == nt;
-        const long long last_unit = item_first + nt - 1;
-        const int c_first = (int)(((item_first + 1) * W + total - 1) / total) - 1;
-        const int c_last = (int)(((last_unit + 1) * W + total - 1) / total) - 1;
+        const bool whole = it.whole();
+        const int c_first = it.first_block(), c_last = it.last_block();
         float* part = parts + ((long long)cta * 2 + (cta == c_first ? 1 : 0)) * C::PART;
         for (int i = tid; i < ROWS * D; i += C::THREADS) {
             const int row = i / D, d = i % D;
@@ -563,8 +354,8 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             if (whole) {
                 if (row < rows) {
                     const int rr = rt * ROWS + row;
-                    const float v = ll > 0.0f || ll != ll ? acc / (ll * a.cache.v_div) * 256.0f : 0.0f;   // scale_pair's 2^-8
-                    a.out[(long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d] = bf16_bits(v);
+                    a.out[(long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d] =
+                        bf16_bits(finish(acc, ll, a.cache.v_div));
                 }
             } else {
                 part[2 * ROWS + i] = acc;
@@ -577,9 +368,9 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
         if (!whole) {
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_find[1] = atomicAdd(&tickets[c_first], 1u) == (uint32_t)(c_last - c_first);
+            if (tid == 0) s_last = atomicAdd(&tickets[c_first], 1u) == (uint32_t)(c_last - c_first);
             __syncthreads();
-            if (s_find[1]) {   // the item's last block: join the parts in token order
+            if (s_last) {   // the item's last block: join the parts in token order
                 __threadfence();
                 if (tid == 0) tickets[c_first] = 0;
                 for (int i = tid; i < rows * D; i += C::THREADS) {
@@ -595,12 +386,11 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
                         mm = v;
                     }
                     const int rr = rt * ROWS + row;
-                    const float v = ll > 0.0f || ll != ll ? acc / (ll * a.cache.v_div) * 256.0f : 0.0f;
-                    a.out[(long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d] = bf16_bits(v);
+                    a.out[(long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d] =
+                        bf16_bits(finish(acc, ll, a.cache.v_div));
                 }
             }
         }
-        u = item_first + k1;
     }
 }
 
@@ -617,37 +407,68 @@ static int attn_sms() {
 }
 
 constexpr int DECODE_WARPS = 8, DECODE_PER_SM = 2;
+// Query rows per kv head and request up to which the decode kernel takes a request.
+constexpr int DECODE_ROWS = 16;
 
-long long kv4_attention_workspace(int heads, int kv_heads, int head_dim) {
-    const long long blocks = (long long)DECODE_PER_SM * attn_sms();
-    return ((blocks * 4 + 255) & ~255LL) + blocks * 2 * 16 * (head_dim + 2) * 4;
+// [decode tickets][prefill tickets][decode parts][prefill parts]; the tickets are zero between calls
+struct WsLayout {
+    int decode_blocks, prefill_blocks;
+    long long prefill_tickets, decode_parts, prefill_parts, bytes;
+};
+static WsLayout ws_layout(int head_dim) {
+    WsLayout w;
+    w.prefill_blocks = attn_sms();
+    w.decode_blocks = DECODE_PER_SM * attn_sms();
+    auto up = [](long long x) { return (x + 255) & ~255LL; };
+    w.prefill_tickets = up(4LL * w.decode_blocks);
+    w.decode_parts = up(w.prefill_tickets + 8LL * w.prefill_blocks);
+    w.prefill_parts = up(w.decode_parts + (long long)w.decode_blocks * 2 * DECODE_ROWS * (head_dim + 2) * 4);
+    w.bytes = w.prefill_parts + kv4_prefill_parts_bytes(w.prefill_blocks, head_dim);
+    return w;
 }
 
+long long kv4_attention_workspace(int head_dim) { return ws_layout(head_dim).bytes; }
+
 template <int D, int NT>
-static int launch_decode(const Kv4AttnArgs& a) {
+static int launch_decode(const Kv4AttnArgs& a, int blocks) {
     using C = DecodeCfg<D, NT, DECODE_WARPS>;
     auto kern = kv4_decode_kernel<D, NT, DECODE_WARPS>;
     static bool ready[64] = {};
     int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return VELOX_ERR_UNSUPPORTED;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return VELOX_ERR_UNSUPPORTED;
     if (!ready[dev]) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
-    EarlyLaunch l((unsigned)(DECODE_PER_SM * attn_sms()), C::THREADS);
+    EarlyLaunch l((unsigned)blocks, C::THREADS);
     l.cfg.dynamicSmemBytes = C::SMEM;
     cudaLaunchKernelEx(&l.cfg, kern, a);
     return launch_status();
 }
 
-int kv4_attention(const Kv4AttnArgs& a) {
+int kv4_attention(Kv4AttnArgs a) {
+    const WsLayout w = ws_layout(a.cache.head_dim);
+    a.prefill_tickets = w.prefill_tickets;
+    a.decode_parts = w.decode_parts;
+    a.prefill_parts = w.prefill_parts;
     const int G = a.heads / a.cache.kv_heads;
-    const long long rows = (long long)a.max_new * G;
-    if (a.cache.head_dim == 128)
-        return rows <= 8 ? launch_decode<128, 1>(a) : launch_decode<128, 2>(a);
-    return rows <= 8 ? launch_decode<64, 1>(a) : launch_decode<64, 2>(a);
+    const long long most = (long long)a.max_new * G;
+    // Two kernels share a call whose requests may be of both kinds; each passes over the other's. (The
+    // lengths are on the device, so the host goes by max_new alone.)
+    if (G <= DECODE_ROWS) {
+        a.min_rows = 0;
+        a.max_rows = DECODE_ROWS;
+        int rc;
+        if (a.cache.head_dim == 128)
+            rc = most <= 8 ? launch_decode<128, 1>(a, w.decode_blocks) : launch_decode<128, 2>(a, w.decode_blocks);
+        else
+            rc = most <= 8 ? launch_decode<64, 1>(a, w.decode_blocks) : launch_decode<64, 2>(a, w.decode_blocks);
+        if (rc != 0 || most <= DECODE_ROWS) return rc;
+    }
+    a.min_rows = G <= DECODE_ROWS ? DECODE_ROWS : 0;
+    a.max_rows = 0x7fffffff;
+    return kv4_prefill(a, w.prefill_blocks);
 }
 
 }  // namespace vx

@@ -1,0 +1,271 @@
+// How the attention kernels cut a step: items (request, kv head, tile of query rows), laid end to
+// end in units of one tile of tokens, an equal run of units per block. The lengths live on the
+// device, so every block finds its run itself.
+#pragma once
+
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace vx {
+
+constexpr float NEG_BIG = -1e30f;   // "no score yet": finite, so that differences of it are numbers
+
+// What a request asks of a kernel.
+struct Request {
+    int row0, n, kv_len, row_tiles;
+    long long units;   // of one kv head
+};
+
+struct RowRange {
+    int lo, hi;   // tokens any of the rows sees
+};
+
+template <int ROWS>
+__device__ __forceinline__ RowRange rows_range(const Kv4AttnArgs& a, int G, const Request& r, int tile) {
+    const int first = r.kv_len - r.n + tile * ROWS / G;
+    const int last = r.kv_len - r.n + (min((tile + 1) * ROWS, r.n * G) - 1) / G;
+    RowRange x;
+    x.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
+    x.hi = a.causal ? min(r.kv_len, last + 1) : r.kv_len;
+    return x;
+}
+
+template <int TILE>
+__device__ __forceinline__ int tiles_of(const RowRange& x) {
+    // an item that sees nothing still has one tile: its rows get zeros
+    return x.hi <= x.lo ? 1 : (x.hi + TILE - 1) / TILE - x.lo / TILE;
+}
+
+// Requests with more new rows than the caller's hint, or with a number of query rows per kv head
+// outside (min_rows, max_rows] (another kernel's), have no units.
+template <int ROWS, int TILE>
+__device__ __forceinline__ Request request_of(const Kv4AttnArgs& a, int G, int b) {
+    Request r;
+    r.row0 = min(max(a.cu[b], 0), a.tokens);
+    r.n = max(0, min(max(a.cu[b + 1], 0), a.tokens) - r.row0);
+    r.kv_len = (int)min((long long)max(a.kv_lens[b], 0), (long long)a.cols * a.cache.page_size);
+    if (r.n > a.max_new || (long long)r.n * G <= a.min_rows || (long long)r.n * G > a.max_rows) r.n = 0;
+    r.row_tiles = (r.n * G + ROWS - 1) / ROWS;
+    r.units = 0;
+    for (int t = 0; t < r.row_tiles; t++) r.units += tiles_of<TILE>(rows_range<ROWS>(a, G, r, t));
+    return r;
+}
+
+// This block's run of units and the request it starts in. Called by all THREADS threads of the
+// block; `red` holds THREADS / 32 words of shared memory, `found` two.
+struct Run {
+    long long total, begin, end, request_first;
+    int blocks;    // blocks that have a run
+    int request;
+};
+template <int ROWS, int TILE, int THREADS>
+__device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* red, long long* found) {
+    constexpr int WARPS = THREADS / 32;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hkv = a.cache.kv_heads;
+    Run run;
+    long long mine = 0;
+    for (int b = tid; b < a.requests; b += THREADS) mine += request_of<ROWS, TILE>(a, G, b).units * hkv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) red[warp] = mine;
+    __syncthreads();
+    run.total = 0;
+    for (int i = 0; i < WARPS; i++) run.total += red[i];
+    run.blocks = (int)min((long long)gridDim.x, run.total);
+    run.request = 0;
+    run.request_first = run.begin = run.end = 0;
+    if ((int)blockIdx.x >= run.blocks) return run;
+    run.begin = run.total * blockIdx.x / run.blocks;
+    run.end = run.total * (blockIdx.x + 1) / run.blocks;
+    long long before = 0;
+    for (int base = 0; base < a.requests; base += THREADS) {
+        const int b = base + tid;
+        const long long v = b < a.requests ? request_of<ROWS, TILE>(a, G, b).units * hkv : 0;
+        long long x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) red[warp] = x;
+        __syncthreads();
+        long long pre = before, sum = 0;
+        for (int i = 0; i < WARPS; i++) {
+            pre += i < warp ? red[i] : 0;
+            sum += red[i];
+        }
+        const long long lo = pre + x - v;
+        if (run.begin >= lo && run.begin < lo + v) {
+            found[0] = b;
+            found[1] = lo;
+        }
+        before += sum;
+        if (before > run.begin) break;
+    }
+    __syncthreads();
+    run.request = (int)found[0];
+    run.request_first = found[1];
+    return run;
+}
+
+// Walks the items of a run.
+template <int ROWS, int TILE>
+struct Items {
+    Request r;
+    RowRange range;
+    long long u, end, req_first, item_first, total;
+    int b, h, rt, nt, k0, k1, blocks;
+
+    __device__ __forceinline__ Items(const Kv4AttnArgs& a, int G, const Run& run)
+        : u(run.begin), end(run.end), req_first(run.request_first), total(run.total), b(run.request), blocks(run.blocks) {
+        if (u < end) r = request_of<ROWS, TILE>(a, G, b);
+    }
+    // The item that holds u; false at the end of the run. done() moves on.
+    __device__ __forceinline__ bool next(const Kv4AttnArgs& a, int G) {
+        if (u >= end) return false;
+        const int hkv = a.cache.kv_heads;
+        while (u >= req_first + r.units * hkv) {   // (requests without rows have no units)
+            req_first += r.units * hkv;
+            r = request_of<ROWS, TILE>(a, G, ++b);
+        }
+        h = (int)((u - req_first) / r.units);
+        item_first = req_first + (long long)h * r.units;
+        rt = 0;
+        range = rows_range<ROWS>(a, G, r, 0);
+        nt = tiles_of<TILE>(range);
+        while (u >= item_first + nt) {
+            item_first += nt;
+            range = rows_range<ROWS>(a, G, r, ++rt);
+            nt = tiles_of<TILE>(range);
+        }
+        k0 = (int)(u - item_first);
+        k1 = (int)min((long long)nt, end - item_first);
+        return true;
+    }
+    __device__ __forceinline__ void done() { u = item_first + k1; }
+    __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nt; }
+    // First and last block that hold a part of this item.
+    __device__ __forceinline__ int first_block() const { return (int)(((item_first + 1) * blocks + total - 1) / total) - 1; }
+    __device__ __forceinline__ int last_block() const { return (int)(((item_first + nt) * blocks + total - 1) / total) - 1; }
+};
+
+// ---- reading the cache -------------------------------------------------------------------------
+
+__device__ __forceinline__ uint4 ldg_stream16(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const uint8_t* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ldg_stream4(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ldg_stream2(const uint8_t* p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+
+// Eight E2M1 codes of a word -> four f16x2 (byte b holds codes 2b, 2b + 1; the first in the low half).
+__device__ __forceinline__ void codes_to_f16(uint32_t word, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(word));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Scale bytes (as seven magnitude bits) to f16, times 2^-8, exactly: the E4M3 pattern moved up seven
+// places is the same number with f16's bias.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t word, uint32_t sel) {   // sel: the two bytes, 0x4x4y
+    return (__byte_perm(word, 0, sel) << 7) & 0x3f803f80u;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A lane's operands of one block of 16 tokens.
+template <int D>
+struct KRegs {
+    uint32_t c[2][D / 32];   // D/4 codes of tokens g and g + 8
+    uint32_t s;
+};
+template <int D>
+struct VRegs {
+    uint32_t c[2][D / 32];   // [p]: tokens 8p + 2t, 8p + 2t + 1, D/8 codes each
+    uint32_t s;
+};
+
+template <int D>
+__device__ __forceinline__ void load_plane(uint32_t (&c)[2][D / 32], const uint8_t* p, int lane) {
+    if (D == 128) {
+        const uint4 x = ldg_stream16(p + lane * 16), y = ldg_stream16(p + 512 + lane * 16);
+        c[0][0] = x.x; c[0][1] = x.y; c[0][D / 32 - 2] = x.z; c[0][D / 32 - 1] = x.w;
+        c[1][0] = y.x; c[1][1] = y.y; c[1][D / 32 - 2] = y.z; c[1][D / 32 - 1] = y.w;
+    } else {
+        const uint2 x = ldg_stream8(p + lane * 8), y = ldg_stream8(p + 256 + lane * 8);
+        c[0][0] = x.x; c[0][1] = x.y;
+        c[1][0] = y.x; c[1][1] = y.y;
+    }
+}
+template <int D>
+__device__ __forceinline__ void load_k(KRegs<D>& r, const uint8_t* blk, int lane) {
+    if (blk == nullptr) {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) r.c[0][i] = r.c[1][i] = 0;
+        r.s = 0;
+        return;
+    }
+    load_plane<D>(r.c, blk, lane);
+    r.s = D == 128 ? ldg_stream4(blk + 16 * D + lane * 4) : ldg_stream2(blk + 16 * D + lane * 2);
+}
+template <int D>
+__device__ __forceinline__ void load_v(VRegs<D>& r, const uint8_t* blk, int lane) {
+    if (blk == nullptr) {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) r.c[0][i] = r.c[1][i] = 0;
+        r.s = 0;
+        return;
+    }
+    load_plane<D>(r.c, blk + 8 * D, lane);
+    // the group of lane (g, t): g where a group is one lane's 16 dimensions, g / 2 where it is two lanes'
+    r.s = ldg_stream4(blk + 17 * D + (D == 128 ? lane : (lane >> 3) * 4 + (lane & 3)) * 4);
+}
+
+// log2 factor of a score: softmax scale, K's divisor, 2^8 for scale_pair's 2^-8.
+__device__ __forceinline__ float score_factor(const Kv4AttnArgs& a) {
+    return a.scale * 1.4426950408889634f / a.cache.k_div * 256.0f;
+}
+// The power of two that brings a row's largest |q| into [1, 2) (a row of zeros, or of numbers below
+// 2^-100, stays as it is), as an exponent.
+__device__ __forceinline__ int row_exponent(float amax) {
+    return min(max((int)(__float_as_uint(amax) >> 23), 27), 227) - 127;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// acc / (sum * divisor), times scale_pair's 2^8; a row that saw nothing (sum 0) is zero.
+__device__ __forceinline__ float finish(float acc, float sum, float v_div) {
+    return sum > 0.0f || sum != sum ? acc / (sum * v_div) * 256.0f : 0.0f;
+}
+
+}  // namespace vx

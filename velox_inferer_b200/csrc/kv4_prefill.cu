@@ -1,0 +1,559 @@
+// Attention over the 4-bit key/value cache for many query rows (prefill chunks, wide groups), on the
+// 5th-generation tensor cores.
+//
+// An item is 256 query rows of one (request, kv head) - new tokens times the group's query heads -
+// against a run of tiles of 128 cached tokens. Per tile
+//   S_w = Q_w K^T       two 128 x 128 products (kind::f16, operands in shared memory),
+//   P_w = 2^(S_w - m)   in registers, one row per thread, back into tensor memory as f16,
+//   O_w += P_w V        two 128 x D products (A from tensor memory),
+// with w the two halves of the rows: while one half is exponentiated the other half's products run.
+// K and V arrive as 4-bit codes; four warps turn each tile into f16 operands in shared memory once
+// for both halves (code * scale is exact), K as rows of D (K-major), V as it lies, token rows (the
+// MMA reads it MN-major, so nothing is transposed). Rows are scaled by powers of two into f16's range as
+// in the decode kernel; P carries a factor 2^6 so that small probabilities stay normal, and the running
+// maximum is only raised, and O rescaled, when it grows by more than 2^8 (P stays below 2^14).
+//
+// Roles of the 16 warps: 0-3 and 4-7 softmax of the two halves (also their Q rows and results), 8-11
+// conversion, 12 issues the MMAs. Tensor memory: S_0, S_1 (P over their first 64 columns), O_0, O_1.
+// Work is cut over the blocks as in the decode kernel (kv4_items.cuh); halves of an item that several
+// blocks share are parked and joined in token order by the last block to arrive.
+#include "common.cuh"
+#include "kv4.cuh"
+#include "kv4_items.cuh"
+#include "tcgen.cuh"
+
+namespace vx {
+
+static __device__ int g_kv4_status = 0;
+enum { KV4_TIMEOUT = 7 };
+
+constexpr int PF_ROWS = 256, PF_TILE = 128, PF_THREADS = 512;
+
+template <int D>
+struct PrefillCfg {
+    static constexpr int PANELS = D / 64;                 // 64 f16 = one 128-byte swizzled row
+    static constexpr int KV_BYTES = PF_TILE * D * 2;      // one operand tile
+    static constexpr int PANEL = PF_TILE * 128;           // bytes of a panel of 128 rows
+    // V first: its descriptors have the largest strides
+    static constexpr int OFF_V = 0, OFF_K = 2 * KV_BYTES, OFF_Q = 4 * KV_BYTES;
+    static constexpr int OFF_BARS = OFF_Q + PF_ROWS * D * 2;
+    static constexpr int SMEM = OFF_BARS + 256 + 1024;    // (aligned by hand to 1024)
+    static constexpr int PART = 128 * (D + 2);            // floats of one parked half
+    static constexpr uint32_t S_COL = 0, O_COL = 256;     // of half 0; half 1: + 128 / + D
+};
+
+// ---- waits that end --------------------------------------------------------------------------------
+// A wait that runs out (2 s) or a block that has given up: the roles go on without waiting, every
+// copy and MMA they still issue stays inside the block's own memory, and the kernel ends.
+struct Waiter {
+    volatile int* dead;
+    __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) const {
+        if (mbar_try_wait(bar, parity)) return;
+        const unsigned long long t0 = global_timer_ns();
+        for (uint32_t spins = 1;; spins++) {
+            if (mbar_try_wait(bar, parity)) return;
+            if ((spins & 63u) == 0) {
+                if (*dead) return;
+                if (global_timer_ns() - t0 > 2000000000ull) {
+                    *dead = 1;
+                    atomicExch(&g_kv4_status, KV4_TIMEOUT);
+                    return;
+                }
+            }
+        }
+    }
+};
+
+// D[128 x N] (+)= A . B, f16 operands, f32 accumulator; A from tensor memory.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Instruction descriptor of kind::f16: f32 accumulator, f16 operands, M = 128.
+__device__ __forceinline__ constexpr uint32_t f16_desc(uint32_t n, bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// V as the B operand, MN-major, 128-byte swizzle: 64 dimensions per 128-byte row, token rows in groups of
+// eight 1024 bytes apart, the next 64 dimensions one panel further.
+__device__ __forceinline__ uint64_t smem_desc_v(uint32_t addr, uint32_t panel) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void half_barrier(int w) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); }
+
+template <int D>
+__global__ void __launch_bounds__(PF_THREADS, 1)
+kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    using C = PrefillCfg<D>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    __shared__ long long s_red[PF_THREADS / 32], s_found[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_dead;
+    __shared__ int s_last[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hkv = a.cache.kv_heads, G = a.heads / hkv, P16 = a.cache.page_size >> 4;
+    const uint32_t bars = base + C::OFF_BARS;
+    auto k_full = [&](int s) { return bars + 8u * s; };
+    auto k_empty = [&](int s) { return bars + 16u + 8u * s; };
+    auto v_full = [&](int s) { return bars + 32u + 8u * s; };
+    auto v_empty = [&](int s) { return bars + 48u + 8u * s; };
+    auto q_full = [&](int w) { return bars + 64u + 8u * w; };
+    auto s_full = [&](int w) { return bars + 80u + 8u * w; };
+    auto p_full = [&](int w) { return bars + 96u + 8u * w; };
+    auto o_full = [&](int w) { return bars + 112u + 8u * w; };
+    auto o_empty = [&](int w) { return bars + 128u + 8u * w; };
+    const uint32_t drained = bars + 144u;
+
+    if (tid == 0) {
+        grid_launch_dependents();
+        s_dead = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(k_full(i), 4);
+            mbar_init(k_empty(i), 1);
+            mbar_init(v_full(i), 4);
+            mbar_init(v_empty(i), 1);
+            mbar_init(q_full(i), 128);
+            mbar_init(s_full(i), 1);
+            mbar_init(p_full(i), 128);
+            mbar_init(o_full(i), 1);
+            mbar_init(o_empty(i), 128);
+        }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    grid_dependency_wait();
+    const Run run = find_run<PF_ROWS, PF_TILE, PF_THREADS>(a, G, s_red, s_found);
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const Waiter wait{&s_dead};
+
+    Items<PF_ROWS, PF_TILE> it(a, G, run);
+    if (warp < 8) {
+        // ---------------- softmax of one half: a row per thread ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;" ::: "memory");
+        const int w = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
+        const uint32_t ts = tmem + lanes + C::S_COL + 128u * w, to = tmem + lanes + C::O_COL + (uint32_t)D * w;
+        const float soft = score_factor(a);
+        uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws + a.prefill_tickets);
+        float* parts = reinterpret_cast<float*>(a.ws + a.prefill_parts);
+        uint32_t ph_s = 0, ph_o = 0;
+        for (; it.next(a, G); it.done()) {
+            const Request& r = it.r;
+            const int rows = min(PF_ROWS, r.n * G - it.rt * PF_ROWS) - 128 * w;   // of this half
+            if (rows <= 0) continue;
+            const int tile0 = it.range.lo / PF_TILE, qbase = r.kv_len - r.n;
+            const int rr = it.rt * PF_ROWS + 128 * w + min(row, rows - 1);
+            const int tok_i = rr / G, head = it.h * G + rr % G;
+
+            // the row's Q: f16, scaled, swizzled
+            float ksc;
+            {
+                const uint16_t* p = a.q + (long long)(r.row0 + tok_i) * a.q_stride + (long long)head * D;
+                uint4 x[D / 8];
+                float amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    x[i] = row < rows ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0);
+                    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u[j] << 16)), fabsf(__uint_as_float(u[j] & 0xffff0000u))));
+                }
+                const int e = row_exponent(amax);
+                const float down = pow2(-e);
+                ksc = fmaxf(soft * pow2(e), 1e-37f);   // (a factor of 0 would turn masked scores into NaN)
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        y[j] = pack_f16(__uint_as_float(u[j] << 16) * down, __uint_as_float(u[j] & 0xffff0000u) * down);
+                    sts16(base + C::OFF_Q + (uint32_t)(w * C::PANELS + i / 8) * C::PANEL + (uint32_t)row * 128u +
+                              (uint32_t)(((i & 7) ^ (row & 7)) << 4),
+                          make_uint4(y[0], y[1], y[2], y[3]));
+                }
+            }
+            proxy_fence();
+            mbar_arrive(q_full(w));
+
+            const int pos = qbase + tok_i;
+            const int lim_hi = a.causal ? min(r.kv_len, pos + 1) : r.kv_len;
+            const int lim_lo = a.window > 0 ? pos - a.window + 1 : 0;
+            // between these every row of the half sees every token
+            const int first_i = (it.rt * PF_ROWS + 128 * w) / G, last_i = (it.rt * PF_ROWS + 128 * w + min(rows, 128) - 1) / G;
+            const int all_hi = a.causal ? min(r.kv_len, qbase + first_i + 1) : r.kv_len;
+            const int all_lo = a.window > 0 ? qbase + last_i - a.window + 1 : 0;
+
+            const int32_t* trow = a.table + (long long)it.b * a.cols;
+            const int blk_hi = (it.range.hi + 15) >> 4;
+            auto pages_there = [&](int k) {   // bit i: block i of the tile lies in the cache
+                const int kb = (tile0 + k) * (PF_TILE / 16) + lane;
+                const int id = lane < 8 && kb < blk_hi ? trow[kb / P16] : -1;
+                return __ballot_sync(0xffffffffu, id >= 0 && id < a.cache.pages);
+            };
+            uint32_t there = pages_there(it.k0);
+            float m = NEG_BIG, l = 0.0f;
+            for (int k = it.k0; k < it.k1; k++) {
+                const uint32_t there_next = k + 1 < it.k1 ? pages_there(k + 1) : 0;
+                wait(s_full(w), ph_s);
+                ph_s ^= 1u;
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc_ld32(ts + 32u * c, s[c]);
+                tc_wait_ld();
+                const int tok = (tile0 + k) * PF_TILE;
+                if (tok < all_lo || tok + PF_TILE > all_hi || there != 0xffu) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const int j = tok + c * 32 + i;
+                            if (j < lim_lo || j >= lim_hi || !(there >> (c * 2 + i / 16) & 1u)) s[c][i] = __float_as_uint(-INFINITY);
+                        }
+                }
+                there = there_next;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        mx = fmaxf(mx, fmaxf(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])));
+                mx *= ksc;
+                if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+                    const float v = fmaxf(m, mx), f = exp2_approx(m - v);
+                    m = v;
+                    l *= f;
+                    if (k > it.k0) {   // (the first tile's product overwrites O)
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            uint32_t o[32];
+                            tc_ld32(to + 32u * c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tc_st32(to + 32u * c, o);
+                        }
+                    }
+                }
+                const float off = 6.0f - m;
+                float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const int j = i * 2;
+                        const float x = exp2_approx(fmaf(__uint_as_float(s[c * 2 + j / 32][j % 32]), ksc, off));
+                        const float y = exp2_approx(fmaf(__uint_as_float(s[c * 2 + j / 32][j % 32 + 1]), ksc, off));
+                        l0 += x;
+                        l1 += y;
+                        p[i] = pack_f16(x, y);
+                    }
+                    tc_st32(ts + 32u * c, p);
+                }
+                l += l0 + l1;
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(p_full(w));
+            }
+
+            // ---- result ----
+            wait(o_full(w), ph_o);
+            ph_o ^= 1u;
+            tc_fence_after();
+            const bool whole = it.whole();
+            const int c_first = it.first_block(), c_last = it.last_block();
+            const int cta = blockIdx.x;
+            uint16_t* dst = a.out + (long long)(r.row0 + tok_i) * a.out_stride + (long long)head * D;
+            float* part = parts + (((long long)cta * 2 + (cta == c_first ? 1 : 0)) * 2 + w) * C::PART;
+            const float inv = finish(1.0f, l, a.cache.v_div);
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t o[32];
+                tc_ld32(to + 32u * c, o);
+                tc_wait_ld();
+                if (whole) {
+                    if (row < rows) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4*>(dst + 32 * c + i) =
+                                make_uint4(pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv),
+                                           pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv),
+                                           pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv),
+                                           pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(part + 256 + ((c * 8 + i / 4) * 128 + row) * 4) =
+                            make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(o_empty(w));
+            if (!whole) {
+                part[row] = m;
+                part[128 + row] = l;
+                __threadfence();
+                half_barrier(w);
+                if (row == 0) s_last[w] = atomicAdd(&tickets[c_first * 2 + w], 1u) == (uint32_t)(c_last - c_first);
+                half_barrier(w);
+                if (s_last[w]) {   // the half's last block: join the parts in token order
+                    __threadfence();
+                    if (row == 0) tickets[c_first * 2 + w] = 0;
+                    auto part_of = [&](int c) { return parts + (((long long)c * 2 + (c == c_first ? 1 : 0)) * 2 + w) * C::PART; };
+                    float mm = NEG_BIG, ll = 0.0f;
+                    for (int c = c_first; c <= c_last; c++) mm = fmaxf(mm, __ldcg(part_of(c) + row));
+                    for (int c = c_first; c <= c_last; c++) ll += exp2_approx(__ldcg(part_of(c) + row) - mm) * __ldcg(part_of(c) + 128 + row);
+                    const float inv2 = finish(1.0f, ll, a.cache.v_div);
+                    for (int d = 0; d < D; d += 8) {
+                        float o[8] = {};
+                        for (int c = c_first; c <= c_last; c++) {
+                            const float* q = part_of(c);
+                            const float f = exp2_approx(__ldcg(q + row) - mm);
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(q + 256 + ((d / 4) * 128 + row) * 4));
+                            const float4 y = __ldcg(reinterpret_cast<const float4*>(q + 256 + ((d / 4 + 1) * 128 + row) * 4));
+                            o[0] += f * x.x; o[1] += f * x.y; o[2] += f * x.z; o[3] += f * x.w;
+                            o[4] += f * y.x; o[5] += f * y.y; o[6] += f * y.z; o[7] += f * y.w;
+                        }
+                        if (row < rows)
+                            *reinterpret_cast<uint4*>(dst + d) = make_uint4(pack_bf16(o[0] * inv2, o[1] * inv2), pack_bf16(o[2] * inv2, o[3] * inv2),
+                                                                            pack_bf16(o[4] * inv2, o[5] * inv2), pack_bf16(o[6] * inv2, o[7] * inv2));
+                    }
+                }
+                half_barrier(w);   // (s_last)
+            }
+        }
+    } else if (warp < 12) {
+        // ---------------- 4-bit tiles to f16 operands ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+        const int g = lane >> 2, t = lane & 3, wq = warp - 8;
+        int n = 0;   // tiles so far: stage n & 1, its use n >> 1
+        for (; it.next(a, G); it.done()) {
+            const int tile0 = it.range.lo / PF_TILE, h = it.h;
+            const int32_t* trow = a.table + (long long)it.b * a.cols;
+            const int blk_hi = (it.range.hi + 15) >> 4;
+            auto page_of = [&](int k) {   // lane i: block i & 1 of this warp in tile k + i / 2
+                const int kb = (tile0 + k + (lane >> 1)) * (PF_TILE / 16) + wq * 2 + (lane & 1);
+                return kb < blk_hi && k + (lane >> 1) < it.k1 ? trow[kb / P16] : -1;
+            };
+            auto block_at = [&](int id, int k, int which) -> const uint8_t* {
+                if (id < 0 || id >= a.cache.pages) return nullptr;
+                const int kb = (tile0 + k) * (PF_TILE / 16) + wq * 2 + which;
+                return a.cache.blocks + (((long long)id * hkv + h) * P16 + kb % P16) * (18 * D);
+            };
+            int ids = page_of(it.k0), ids_at = it.k0;
+            const uint8_t* blk[2];
+            KRegs<D> kr[2];
+            VRegs<D> vr[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                blk[i] = block_at(__shfl_sync(0xffffffffu, ids, i), it.k0, i);
+                load_k<D>(kr[i], blk[i], lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) load_v<D>(vr[i], blk[i], lane);
+            for (int k = it.k0; k < it.k1; k++, n++) {
+                const int st = n & 1;
+                const uint32_t ph = ((uint32_t)(n >> 1) & 1u) ^ 1u;
+                wait(k_empty(st), ph);
+                // K: lane (g, t) has tokens g and g + 8, dimensions t*D/4 ..: D/32 words of eight dimensions, one
+                // 16-byte chunk each. In lanes t >= 2 the words are taken in another order (w ^ D/64), so that the
+                // eight lanes of a store phase write eight different chunk positions.
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int hh = 0; hh < 2; hh++) {
+                        const int tau = (wq * 2 + i) * 16 + hh * 8 + g;
+                        const uint32_t rowp = base + C::OFF_K + (uint32_t)st * C::KV_BYTES + (uint32_t)tau * 128u;
+                        const uint32_t b0 = (D == 128 ? kr[i].s >> (16 * hh) : kr[i].s >> (8 * hh)) & 0xffu;
+                        const uint32_t b1 = D == 128 ? kr[i].s >> (16 * hh + 8) & 0xffu : b0;
+                        const uint32_t sc[2] = {((b0 | b0 << 16) << 7) & 0x3f803f80u, ((b1 | b1 << 16) << 7) & 0x3f803f80u};
+                        constexpr int W = D / 32;
+                        const bool flip = t >= 2;
+#pragma unroll
+                        for (int x = 0; x < W; x++) {
+                            const uint32_t word = flip ? kr[i].c[hh][x ^ (W / 2)] : kr[i].c[hh][x];
+                            // (a scale covers 16 dimensions = two words)
+                            const uint32_t s = W == 2 ? sc[0] : (flip ? sc[(x ^ (W / 2)) / 2] : sc[x / 2]);
+                            uint32_t f[4];
+                            codes_to_f16(word, f);
+                            const int dim8 = t * W + (flip ? x ^ (W / 2) : x);   // eighth of the row
+                            sts16(rowp + (uint32_t)(dim8 >> 3) * C::PANEL + (uint32_t)(((dim8 & 7) ^ (tau & 7)) << 4),
+                                  make_uint4(mul_f16x2(f[0], s), mul_f16x2(f[1], s), mul_f16x2(f[2], s), mul_f16x2(f[3], s)));
+                        }
+                    }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full(st));
+                if (k + 1 < it.k1) {
+                    if (k + 1 - ids_at == 16) {
+                        ids_at = k + 1;
+                        ids = page_of(ids_at);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        blk[i] = block_at(__shfl_sync(0xffffffffu, ids, (k + 1 - ids_at) * 2 + i), k + 1, i);
+                        load_k<D>(kr[i], blk[i], lane);
+                    }
+                }
+                wait(v_empty(st), ph);
+                // V: lane (g, t) has tokens 8p + 2t + j, dimensions g*D/8 ..: D/64 chunks of eight dimensions per token;
+                // chunk order flipped in odd lane groups (D = 128) for the same reason.
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int p = 0; p < 2; p++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            constexpr int W = D / 64;
+                            const int tau = (wq * 2 + i) * 16 + p * 8 + 2 * t + j;
+                            const uint32_t rowp = base + C::OFF_V + (uint32_t)st * C::KV_BYTES + (uint32_t)tau * 128u;
+                            const uint32_t bs = vr[i].s >> (16 * p + 8 * j) & 0xffu;
+                            const uint32_t s = ((bs | bs << 16) << 7) & 0x3f803f80u;
+                            const bool flip = W == 2 && (g & 1);
+#pragma unroll
+                            for (int x = 0; x < W; x++) {
+                                const uint32_t word = flip ? vr[i].c[p][j * W + (x ^ (W - 1))] : vr[i].c[p][j * W + x];
+                                uint32_t f[4];
+                                codes_to_f16(word, f);
+                                const int dim8 = g * W + (flip ? x ^ (W - 1) : x);
+                                sts16(rowp + (uint32_t)(dim8 >> 3) * C::PANEL + (uint32_t)(((dim8 & 7) ^ (tau & 7)) << 4),
+                                      make_uint4(mul_f16x2(f[0], s), mul_f16x2(f[1], s), mul_f16x2(f[2], s), mul_f16x2(f[3], s)));
+                            }
+                        }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_full(st));
+                if (k + 1 < it.k1) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) load_v<D>(vr[i], blk[i], lane);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
+        if (warp == 12) {
+            // ---------------- MMA issue (the whole warp walks the loop, one lane issues) ----------------
+            const bool leader = elect_one();
+            const uint32_t idesc_s = f16_desc(128, false), idesc_o = f16_desc(D, true);
+            int n = 0;
+            uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0}, items[2] = {0, 0};
+            auto product_s = [&](int w, int st) {
+#pragma unroll
+                for (int pd = 0; pd < C::PANELS; pd++) {
+                    const uint64_t da = smem_desc_sw128(base + C::OFF_Q + (uint32_t)(w * C::PANELS + pd) * C::PANEL);
+                    const uint64_t db = smem_desc_sw128(base + C::OFF_K + (uint32_t)st * C::KV_BYTES + (uint32_t)pd * C::PANEL);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        tc_mma<KIND_BF16, 1>(tmem + C::S_COL + 128u * w, da + 2u * j, db + 2u * j, idesc_s, pd + j > 0 ? 1u : 0u, 0, 0);
+                }
+            };
+            auto product_o = [&](int w, int st, bool fresh) {
+                const uint64_t db = smem_desc_v(base + C::OFF_V + (uint32_t)st * C::KV_BYTES, C::PANEL);
+#pragma unroll
+                for (int j = 0; j < 8; j++)   // sixteen tokens each
+                    tc_mma_f16_ts(tmem + C::O_COL + (uint32_t)D * w, tmem + C::S_COL + 128u * w + 8u * j, db + 128u * j, idesc_o,
+                                  fresh && j == 0 ? 0u : 1u);
+            };
+            for (; it.next(a, G); it.done()) {
+                const int halves = it.r.n * G - it.rt * PF_ROWS > 128 ? 2 : 1;
+                const int count = it.k1 - it.k0;
+                wait(k_full(n & 1), (uint32_t)(n >> 1) & 1u);
+                for (int w = 0; w < halves; w++) {
+                    wait(q_full(w), ph_q[w]);
+                    ph_q[w] ^= 1u;
+                    tc_fence_after();
+                    if (leader) {
+                        product_s(w, n & 1);
+                        tc_commit(s_full(w));
+                        if (w == halves - 1) tc_commit(k_empty(n & 1));
+                    }
+                }
+                for (int i = 0; i < count; i++, n++) {
+                    const int st = n & 1, nx = (n + 1) & 1;
+                    const bool more = i + 1 < count;
+                    wait(v_full(st), (uint32_t)(n >> 1) & 1u);
+                    for (int w = 0; w < halves; w++) {
+                        wait(p_full(w), ph_p[w]);
+                        ph_p[w] ^= 1u;
+                        if (i == 0) {
+                            wait(o_empty(w), (items[w] & 1u) ^ 1u);
+                            items[w]++;
+                        }
+                        if (w == 0 && more) wait(k_full(nx), (uint32_t)((n + 1) >> 1) & 1u);
+                        tc_fence_after();
+                        if (leader) {
+                            product_o(w, st, i == 0);
+                            if (w == halves - 1) tc_commit(v_empty(st));
+                            if (more) {
+                                product_s(w, nx);
+                                tc_commit(s_full(w));
+                                if (w == halves - 1) tc_commit(k_empty(nx));
+                            } else {
+                                tc_commit(o_full(w));
+                            }
+                        }
+                    }
+                }
+            }
+            if (leader) tc_commit(drained);   // nothing of this block is in flight when tensor memory is freed
+            wait(drained, 0);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+long long kv4_prefill_parts_bytes(int blocks, int head_dim) { return (long long)blocks * 4 * 128 * (head_dim + 2) * 4; }
+
+template <int D>
+static int launch_prefill(const Kv4AttnArgs& a, int blocks) {
+    using C = PrefillCfg<D>;
+    static bool ready[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return VELOX_ERR_UNSUPPORTED;
+    if (!ready[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return (int)e;
+        ready[dev] = true;
+    }
+    EarlyLaunch l((unsigned)blocks, PF_THREADS);
+    l.cfg.dynamicSmemBytes = C::SMEM;
+    cudaLaunchKernelEx(&l.cfg, kv4_prefill_kernel<D>, a);
+    return launch_status();
+}
+
+int kv4_prefill(const Kv4AttnArgs& a, int blocks) {
+    return a.cache.head_dim == 128 ? launch_prefill<128>(a, blocks) : launch_prefill<64>(a, blocks);
+}
+
+int kv4_status_sync() {
+    int v = -1;
+    if (cudaMemcpyFromSymbol(&v, g_kv4_status, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}
+
+int kv4_status_reset() {
+    const int zero = 0;
+    return (int)cudaMemcpyToSymbol(g_kv4_status, &zero, sizeof(int));
+}
+
+}  // namespace vx
