@@ -131,7 +131,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     float* parts = reinterpret_cast<float*>(a.ws + a.decode_parts);
 
     Items<ROWS, TILE> it(a, G, run);
-    for (; it.next(a, G); it.done()) {
+    for (; it.more(); it.next(a, G)) {
         const Request& r = it.r;
         const RowRange range = it.range;
         const int b = it.b, h = it.h, rt = it.rt, k0 = it.k0, k1 = it.k1;

@@ -21,12 +21,10 @@ struct RowRange {
 };
 
 template <int ROWS>
-__device__ __forceinline__ RowRange rows_range(const Kv4AttnArgs& a, int G, const Request& r, int tile) {
-    const int first = r.kv_len - r.n + tile * ROWS / G;
-    const int last = r.kv_len - r.n + (min((tile + 1) * ROWS, r.n * G) - 1) / G;
+__device__ __forceinline__ RowRange rows_range(const Kv4AttnArgs& a, int G, int n, int kv_len, int tile) {
     RowRange x;
-    x.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-    x.hi = a.causal ? min(r.kv_len, last + 1) : r.kv_len;
+    x.lo = a.window > 0 ? max(0, kv_len - n + tile * ROWS / G - a.window + 1) : 0;
+    x.hi = a.causal ? min(kv_len, kv_len - n + (min((tile + 1) * ROWS, n * G) - 1) / G + 1) : kv_len;
     return x;
 }
 
@@ -37,8 +35,8 @@ __device__ __forceinline__ int tiles_of(const RowRange& x) {
 }
 
 // Requests with more new rows than the caller's hint, or with a number of query rows per kv head
-// outside (min_rows, max_rows] (another kernel's), have no units.
-template <int ROWS, int TILE>
+// outside (min_rows, max_rows] (another kernel's), have no rows here. `units` is left to the caller.
+template <int ROWS>
 __device__ __forceinline__ Request request_of(const Kv4AttnArgs& a, int G, int b) {
     Request r;
     r.row0 = min(max(a.cu[b], 0), a.tokens);
@@ -46,9 +44,33 @@ __device__ __forceinline__ Request request_of(const Kv4AttnArgs& a, int G, int b
     r.kv_len = (int)min((long long)max(a.kv_lens[b], 0), (long long)a.cols * a.cache.page_size);
     if (r.n > a.max_new || (long long)r.n * G <= a.min_rows || (long long)r.n * G > a.max_rows) r.n = 0;
     r.row_tiles = (r.n * G + ROWS - 1) / ROWS;
-    r.units = 0;
-    for (int t = 0; t < r.row_tiles; t++) r.units += tiles_of<TILE>(rows_range<ROWS>(a, G, r, t));
     return r;
+}
+
+// Units of one kv head of a request, by the whole warp (the same request in every lane).
+template <int ROWS, int TILE>
+__device__ __forceinline__ long long warp_units(const Kv4AttnArgs& a, int G, int n, int kv_len, int row_tiles) {
+    long long sum = 0;
+    for (int t = threadIdx.x & 31; t < row_tiles; t += 32) sum += tiles_of<TILE>(rows_range<ROWS>(a, G, n, kv_len, t));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+// The same for a request per lane: a lane counts a single row tile itself, the warp together counts the others'.
+template <int ROWS, int TILE>
+__device__ __forceinline__ long long lane_units(const Kv4AttnArgs& a, int G, int b) {
+    Request r{};
+    if (b < a.requests) r = request_of<ROWS>(a, G, b);
+    long long units = r.row_tiles == 1 ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0;
+    uint32_t many = __ballot_sync(0xffffffffu, r.row_tiles > 1);
+    while (many) {
+        const int src = __ffs(many) - 1;
+        many &= many - 1;
+        const long long u = warp_units<ROWS, TILE>(a, G, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.kv_len, src),
+                                                   __shfl_sync(0xffffffffu, r.row_tiles, src));
+        if ((threadIdx.x & 31) == src) units = u;
+    }
+    return units;
 }
 
 // This block's run of units and the request it starts in. Called by all THREADS threads of the
@@ -63,13 +85,18 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hkv = a.cache.kv_heads;
     Run run;
-    long long mine = 0;
-    for (int b = tid; b < a.requests; b += THREADS) mine += request_of<ROWS, TILE>(a, G, b).units * hkv;
+    const bool once = a.requests <= THREADS;
+    long long first = 0, mine = 0;
+    for (int base = 0; base < a.requests; base += THREADS) {
+        first = lane_units<ROWS, TILE>(a, G, base + tid) * hkv;
+        mine += first;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) red[warp] = mine;
     __syncthreads();
     run.total = 0;
+#pragma unroll
     for (int i = 0; i < WARPS; i++) run.total += red[i];
     run.blocks = (int)min((long long)gridDim.x, run.total);
     run.request = 0;
@@ -80,17 +107,20 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     long long before = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
         const int b = base + tid;
-        const long long v = b < a.requests ? request_of<ROWS, TILE>(a, G, b).units * hkv : 0;
+        const long long v = once ? first : lane_units<ROWS, TILE>(a, G, b) * hkv;
         long long x = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        __syncthreads();
-        if (lane == 31) red[warp] = x;
-        __syncthreads();
+        if (!once) {
+            __syncthreads();
+            if (lane == 31) red[warp] = x;
+            __syncthreads();
+        }
         long long pre = before, sum = 0;
+#pragma unroll
         for (int i = 0; i < WARPS; i++) {
             pre += i < warp ? red[i] : 0;
             sum += red[i];
@@ -109,41 +139,73 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     return run;
 }
 
-// Walks the items of a run.
+// Walks the items of a run. Called by whole warps.
 template <int ROWS, int TILE>
 struct Items {
     Request r;
     RowRange range;
-    long long u, end, req_first, item_first, total;
+    long long u, end, item_first, total;
     int b, h, rt, nt, k0, k1, blocks;
 
     __device__ __forceinline__ Items(const Kv4AttnArgs& a, int G, const Run& run)
-        : u(run.begin), end(run.end), req_first(run.request_first), total(run.total), b(run.request), blocks(run.blocks) {
-        if (u < end) r = request_of<ROWS, TILE>(a, G, b);
-    }
-    // The item that holds u; false at the end of the run. done() moves on.
-    __device__ __forceinline__ bool next(const Kv4AttnArgs& a, int G) {
-        if (u >= end) return false;
-        const int hkv = a.cache.kv_heads;
-        while (u >= req_first + r.units * hkv) {   // (requests without rows have no units)
-            req_first += r.units * hkv;
-            r = request_of<ROWS, TILE>(a, G, ++b);
-        }
-        h = (int)((u - req_first) / r.units);
-        item_first = req_first + (long long)h * r.units;
+        : u(run.begin), end(run.end), total(run.total), b(run.request), blocks(run.blocks) {
+        if (u >= end) return;
+        load(a, G);
+        h = (int)((u - run.request_first) / r.units);
+        item_first = run.request_first + (long long)h * r.units;
         rt = 0;
-        range = rows_range<ROWS>(a, G, r, 0);
-        nt = tiles_of<TILE>(range);
-        while (u >= item_first + nt) {
-            item_first += nt;
-            range = rows_range<ROWS>(a, G, r, ++rt);
-            nt = tiles_of<TILE>(range);
+        if (r.row_tiles > 1) {   // the row tile that holds u: 32 at a time
+            const int lane = threadIdx.x & 31;
+            for (;; rt += 32) {
+                const int t = rt + lane;
+                const int v = t < r.row_tiles ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, t)) : 0;
+                int x = v;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, x, o);
+                    if (lane >= o) x += y;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, item_first + x > u);
+                const int at = past ? __ffs(past) - 1 : 31;
+                const int upto = __shfl_sync(0xffffffffu, x, at), size = __shfl_sync(0xffffffffu, v, at);
+                if (past) {
+                    item_first += upto - size;
+                    rt += at;
+                    break;
+                }
+                item_first += upto;
+            }
         }
+        enter(a, G);
+    }
+    __device__ __forceinline__ void load(const Kv4AttnArgs& a, int G) {
+        r = request_of<ROWS>(a, G, b);
+        r.units = r.row_tiles <= 1 ? (r.row_tiles ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0)
+                                   : warp_units<ROWS, TILE>(a, G, r.n, r.kv_len, r.row_tiles);
+    }
+    __device__ __forceinline__ void enter(const Kv4AttnArgs& a, int G) {
+        range = rows_range<ROWS>(a, G, r.n, r.kv_len, rt);
+        nt = tiles_of<TILE>(range);
         k0 = (int)(u - item_first);
         k1 = (int)min((long long)nt, end - item_first);
-        return true;
     }
-    __device__ __forceinline__ void done() { u = item_first + k1; }
+    __device__ __forceinline__ bool more() const { return u < end; }
+    __device__ __forceinline__ void next(const Kv4AttnArgs& a, int G) {
+        item_first += nt;
+        u = item_first;
+        if (u >= end) return;
+        if (++rt == r.row_tiles) {
+            rt = 0;
+            if (++h == a.cache.kv_heads) {
+                h = 0;
+                do {   // (requests without rows have no units; there is one with units, since u < end)
+                    b++;
+                    load(a, G);
+                } while (r.units == 0);
+            }
+        }
+        enter(a, G);
+    }
     __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nt; }
     // First and last block that hold a part of this item.
     __device__ __forceinline__ int first_block() const { return (int)(((item_first + 1) * blocks + total - 1) / total) - 1; }

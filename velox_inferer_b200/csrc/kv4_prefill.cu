@@ -14,7 +14,7 @@
 // maximum is only raised, and O rescaled, when it grows by more than 2^8 (P stays below 2^14).
 //
 // Roles of the 16 warps: 0-3 and 4-7 softmax of the two halves (also their Q rows and results), 8-11
-// conversion, 12 issues the MMAs. Tensor memory: S_0, S_1 (P over their first 64 columns), O_0, O_1.
+// conversion, 12 issues the MMAs. Tensor memory: S_0, S_1 (P over their last 64 columns), O_0, O_1.
 // Work is cut over the blocks as in the decode kernel (kv4_items.cuh); halves of an item that several
 // blocks share are parked and joined in token order by the last block to arrive.
 #include "common.cuh"
@@ -38,8 +38,10 @@ struct PrefillCfg {
     static constexpr int OFF_V = 0, OFF_K = 2 * KV_BYTES, OFF_Q = 4 * KV_BYTES;
     static constexpr int OFF_BARS = OFF_Q + PF_ROWS * D * 2;
     static constexpr int SMEM = OFF_BARS + 256 + 1024;    // (aligned by hand to 1024)
+    static constexpr int RING = 4;                        // items the scheduling warp is ahead
     static constexpr int PART = 128 * (D + 2);            // floats of one parked half
     static constexpr uint32_t S_COL = 0, O_COL = 256;     // of half 0; half 1: + 128 / + D
+    static constexpr uint32_t P_COL = 64;                 // P inside S
 };
 
 // ---- waits that end --------------------------------------------------------------------------------
@@ -82,8 +84,34 @@ __device__ __forceinline__ uint64_t smem_desc_v(uint32_t addr, uint32_t panel) {
     return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Waits for this thread's tensor-memory loads; the registers of `r` pass through, so nothing that uses them can be
+// moved ahead of the wait.
+__device__ __forceinline__ void tc_wait_ld_of(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void half_barrier(int w) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); }
+
+// An item as the roles see it.
+struct PrefillItem {
+    int k0, k1;              // its tiles in this block; k1 = 0: no more items
+    int tile0, hi;           // first tile, end of the tokens any row sees
+    int b, h, row0, first;   // request, kv head, the request's first row, first query row (token * G + head) of the item
+    int rows, n, kv_len;     // query rows of the item; the request's new and all tokens
+    int c_first, c_last;     // blocks that hold parts of it (equal: this one alone)
+    int pad[3];
+};
 
 template <int D>
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -95,6 +123,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
     __shared__ int s_last[2];
+    __shared__ PrefillItem s_items[C::RING];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hkv = a.cache.kv_heads, G = a.heads / hkv, P16 = a.cache.page_size >> 4;
     const uint32_t bars = base + C::OFF_BARS;
@@ -108,6 +137,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     auto o_full = [&](int w) { return bars + 112u + 8u * w; };
     auto o_empty = [&](int w) { return bars + 128u + 8u * w; };
     const uint32_t drained = bars + 144u;
+    auto p_half = [&](int w) { return bars + 216u + 8u * w; };   // the last 64 tokens of P
+    auto item_full = [&](int i) { return bars + 152u + 8u * i; };
+    auto item_empty = [&](int i) { return bars + 184u + 8u * i; };
 
     if (tid == 0) {
         grid_launch_dependents();
@@ -119,11 +151,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             mbar_init(v_empty(i), 1);
             mbar_init(q_full(i), 128);
             mbar_init(s_full(i), 1);
+            mbar_init(p_half(i), 128);
             mbar_init(p_full(i), 128);
             mbar_init(o_full(i), 1);
             mbar_init(o_empty(i), 128);
         }
         mbar_init(drained, 1);
+        for (int i = 0; i < C::RING; i++) {
+            mbar_init(item_full(i), 1);
+            mbar_init(item_empty(i), 13);   // eight softmax warps, four converting, one issuing
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -139,7 +176,19 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     const uint32_t tmem = s_tmem;
     const Waiter wait{&s_dead};
 
-    Items<PF_ROWS, PF_TILE> it(a, G, run);
+    // every warp that works takes the items in turn; they stay in shared memory until it gives them back
+    int item_no = 0;
+    auto take = [&]() -> const PrefillItem* {
+        const int i = item_no % C::RING;
+        wait(item_full(i), (uint32_t)(item_no / C::RING) & 1u);
+        return s_items[i].k1 > 0 && !*wait.dead ? &s_items[i] : nullptr;
+    };
+    auto give_back = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty(item_no % C::RING));
+        item_no++;
+    };
+
     if (warp < 8) {
         // ---------------- softmax of one half: a row per thread ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;" ::: "memory");
@@ -150,18 +199,18 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
         uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws + a.prefill_tickets);
         float* parts = reinterpret_cast<float*>(a.ws + a.prefill_parts);
         uint32_t ph_s = 0, ph_o = 0;
-        for (; it.next(a, G); it.done()) {
-            const Request& r = it.r;
-            const int rows = min(PF_ROWS, r.n * G - it.rt * PF_ROWS) - 128 * w;   // of this half
+        for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
+            const PrefillItem& it = *item;
+            const int rows = it.rows - 128 * w;   // of this half
             if (rows <= 0) continue;
-            const int tile0 = it.range.lo / PF_TILE, qbase = r.kv_len - r.n;
-            const int rr = it.rt * PF_ROWS + 128 * w + min(row, rows - 1);
+            const int tile0 = it.tile0, qbase = it.kv_len - it.n;
+            const int rr = it.first + 128 * w + min(row, rows - 1);
             const int tok_i = rr / G, head = it.h * G + rr % G;
 
             // the row's Q: f16, scaled, swizzled
             float ksc;
             {
-                const uint16_t* p = a.q + (long long)(r.row0 + tok_i) * a.q_stride + (long long)head * D;
+                const uint16_t* p = a.q + (long long)(it.row0 + tok_i) * a.q_stride + (long long)head * D;
                 uint4 x[D / 8];
                 float amax = 0.0f;
 #pragma unroll
@@ -191,48 +240,72 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             mbar_arrive(q_full(w));
 
             const int pos = qbase + tok_i;
-            const int lim_hi = a.causal ? min(r.kv_len, pos + 1) : r.kv_len;
+            const int lim_hi = a.causal ? min(it.kv_len, pos + 1) : it.kv_len;
             const int lim_lo = a.window > 0 ? pos - a.window + 1 : 0;
             // between these every row of the half sees every token
-            const int first_i = (it.rt * PF_ROWS + 128 * w) / G, last_i = (it.rt * PF_ROWS + 128 * w + min(rows, 128) - 1) / G;
-            const int all_hi = a.causal ? min(r.kv_len, qbase + first_i + 1) : r.kv_len;
+            const int first_i = (it.first + 128 * w) / G, last_i = (it.first + 128 * w + min(rows, 128) - 1) / G;
+            const int all_hi = a.causal ? min(it.kv_len, qbase + first_i + 1) : it.kv_len;
             const int all_lo = a.window > 0 ? qbase + last_i - a.window + 1 : 0;
 
             const int32_t* trow = a.table + (long long)it.b * a.cols;
-            const int blk_hi = (it.range.hi + 15) >> 4;
-            auto pages_there = [&](int k) {   // bit i: block i of the tile lies in the cache
+            const int blk_hi = (it.hi + 15) >> 4;
+            // Which of the next four tiles' 32 blocks lie in the cache: the ids are read four tiles ahead.
+            auto page_id = [&](int k) {
                 const int kb = (tile0 + k) * (PF_TILE / 16) + lane;
-                const int id = lane < 8 && kb < blk_hi ? trow[kb / P16] : -1;
-                return __ballot_sync(0xffffffffu, id >= 0 && id < a.cache.pages);
+                return kb < blk_hi ? trow[kb / P16] : -1;
             };
-            uint32_t there = pages_there(it.k0);
+            int ids = page_id(it.k0);
+            uint32_t there4 = 0;
             float m = NEG_BIG, l = 0.0f;
             for (int k = it.k0; k < it.k1; k++) {
-                const uint32_t there_next = k + 1 < it.k1 ? pages_there(k + 1) : 0;
+                if (((k - it.k0) & 3) == 0) {
+                    there4 = __ballot_sync(0xffffffffu, ids >= 0 && ids < a.cache.pages);
+                    ids = page_id(k + 4);
+                }
+                const uint32_t there = there4 & 0xffu;
+                there4 >>= 8;
                 wait(s_full(w), ph_s);
                 ph_s ^= 1u;
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ld32(ts + 32u * c, s[c]);
-                tc_wait_ld();
+                // Scores in four chunks of 32 columns: 0 and 1 are read for the maximum and once more for the
+                // exponentials, 2 and 3 stay in registers in between. (All 128 at once spill, and with nearly
+                // all of the L1 given to operands a spilled register comes back from L2.)
                 const int tok = (tile0 + k) * PF_TILE;
-                if (tok < all_lo || tok + PF_TILE > all_hi || there != 0xffu) {
+                const bool edge = tok < all_lo || tok + PF_TILE > all_hi || there != 0xffu;
+                auto mask = [&](uint32_t (&s)[32], int c) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int i = 0; i < 32; i++) {
+                        const int j = tok + c * 32 + i;
+                        if (j < lim_lo || j >= lim_hi || !(there >> (c * 2 + i / 16) & 1u)) s[i] = __float_as_uint(-INFINITY);
+                    }
+                };
+                auto max32 = [&](const uint32_t (&s)[32]) {
+                    float u = __uint_as_float(s[0]), v = __uint_as_float(s[1]);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int j = tok + c * 32 + i;
-                            if (j < lim_lo || j >= lim_hi || !(there >> (c * 2 + i / 16) & 1u)) s[c][i] = __float_as_uint(-INFINITY);
-                        }
+                    for (int i = 2; i < 30; i += 4) {
+                        u = max3(u, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        v = max3(v, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                    }
+                    return fmaxf(u, max3(v, __uint_as_float(s[30]), __uint_as_float(s[31])));
+                };
+                uint32_t x0[32], x1[32], x2[32];
+                tc_ld32(ts, x0);
+                tc_ld32(ts + 32u, x1);
+                tc_ld32(ts + 64u, x2);
+                tc_wait_ld_of(x0);
+                tc_wait_ld_of(x1);
+                tc_wait_ld_of(x2);
+                if (edge) {
+                    mask(x0, 0);
+                    mask(x1, 1);
+                    mask(x2, 2);
                 }
-                there = there_next;
-                float mx = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        mx = fmaxf(mx, fmaxf(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])));
+                float mx = fmaxf(max32(x0), max32(x1));
+                tc_ld32(ts + 96u, x1);
+                mx = fmaxf(mx, max32(x2));
+                tc_wait_ld_of(x1);
+                if (edge) mask(x1, 3);
+                mx = fmaxf(mx, max32(x1));
                 mx *= ksc;
                 if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
                     const float v = fmaxf(m, mx), f = exp2_approx(m - v);
@@ -243,7 +316,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
                             tc_ld32(to + 32u * c, o);
-                            tc_wait_ld();
+                            tc_wait_ld_of(o);
 #pragma unroll
                             for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                             tc_st32(to + 32u * c, o);
@@ -252,20 +325,35 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 }
                 const float off = 6.0f - m;
                 float l0 = 0.0f, l1 = 0.0f;
+                // P over the second half of S: what a chunk's probabilities overwrite has been read. The product
+                // over the last 64 tokens starts while the first are still being exponentiated.
+                auto chunk = [&](const uint32_t (&s)[32], int c) {
+                    uint32_t p[16];
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const int j = i * 2;
-                        const float x = exp2_approx(fmaf(__uint_as_float(s[c * 2 + j / 32][j % 32]), ksc, off));
-                        const float y = exp2_approx(fmaf(__uint_as_float(s[c * 2 + j / 32][j % 32 + 1]), ksc, off));
+                    for (int i = 0; i < 16; i++) {
+                        const float x = exp2_approx(fmaf(__uint_as_float(s[2 * i]), ksc, off));
+                        const float y = exp2_approx(fmaf(__uint_as_float(s[2 * i + 1]), ksc, off));
                         l0 += x;
                         l1 += y;
                         p[i] = pack_f16(x, y);
                     }
-                    tc_st32(ts + 32u * c, p);
+                    tc_st16(ts + C::P_COL + 16u * c, p);
+                };
+                tc_ld32(ts, x0);
+                chunk(x2, 2);
+                chunk(x1, 3);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(p_half(w));
+                tc_ld32(ts + 32u, x1);
+                tc_wait_ld_of(x0);
+                tc_wait_ld_of(x1);
+                if (edge) {
+                    mask(x0, 0);
+                    mask(x1, 1);
                 }
+                chunk(x0, 0);
+                chunk(x1, 1);
                 l += l0 + l1;
                 tc_wait_st();
                 tc_fence_before();
@@ -276,17 +364,17 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             wait(o_full(w), ph_o);
             ph_o ^= 1u;
             tc_fence_after();
-            const bool whole = it.whole();
-            const int c_first = it.first_block(), c_last = it.last_block();
+            const int c_first = it.c_first, c_last = it.c_last;
+            const bool whole = c_first == c_last;   // (an item split over blocks has two of them at least)
             const int cta = blockIdx.x;
-            uint16_t* dst = a.out + (long long)(r.row0 + tok_i) * a.out_stride + (long long)head * D;
+            uint16_t* dst = a.out + (long long)(it.row0 + tok_i) * a.out_stride + (long long)head * D;
             float* part = parts + (((long long)cta * 2 + (cta == c_first ? 1 : 0)) * 2 + w) * C::PART;
             const float inv = finish(1.0f, l, a.cache.v_div);
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
                 tc_ld32(to + 32u * c, o);
-                tc_wait_ld();
+                tc_wait_ld_of(o);
                 if (whole) {
                     if (row < rows) {
 #pragma unroll
@@ -318,22 +406,37 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     if (row == 0) tickets[c_first * 2 + w] = 0;
                     auto part_of = [&](int c) { return parts + (((long long)c * 2 + (c == c_first ? 1 : 0)) * 2 + w) * C::PART; };
                     float mm = NEG_BIG, ll = 0.0f;
-                    for (int c = c_first; c <= c_last; c++) mm = fmaxf(mm, __ldcg(part_of(c) + row));
-                    for (int c = c_first; c <= c_last; c++) ll += exp2_approx(__ldcg(part_of(c) + row) - mm) * __ldcg(part_of(c) + 128 + row);
+                    for (int c = c_first; c <= c_last; c++) {
+                        const float pm = __ldcg(part_of(c) + row), pl = __ldcg(part_of(c) + 128 + row), v = fmaxf(mm, pm);
+                        ll = ll * exp2_approx(mm - v) + pl * exp2_approx(pm - v);
+                        mm = v;
+                    }
                     const float inv2 = finish(1.0f, ll, a.cache.v_div);
-                    for (int d = 0; d < D; d += 8) {
-                        float o[8] = {};
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 64) {   // sixteen loads in flight per part
+                        float o[64] = {};
+#pragma unroll 1
                         for (int c = c_first; c <= c_last; c++) {
                             const float* q = part_of(c);
+                            float4 x[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[i] = __ldcg(reinterpret_cast<const float4*>(q + 256 + ((d / 4 + i) * 128 + row) * 4));
                             const float f = exp2_approx(__ldcg(q + row) - mm);
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(q + 256 + ((d / 4) * 128 + row) * 4));
-                            const float4 y = __ldcg(reinterpret_cast<const float4*>(q + 256 + ((d / 4 + 1) * 128 + row) * 4));
-                            o[0] += f * x.x; o[1] += f * x.y; o[2] += f * x.z; o[3] += f * x.w;
-                            o[4] += f * y.x; o[5] += f * y.y; o[6] += f * y.z; o[7] += f * y.w;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                o[4 * i] += f * x[i].x;
+                                o[4 * i + 1] += f * x[i].y;
+                                o[4 * i + 2] += f * x[i].z;
+                                o[4 * i + 3] += f * x[i].w;
+                            }
                         }
-                        if (row < rows)
-                            *reinterpret_cast<uint4*>(dst + d) = make_uint4(pack_bf16(o[0] * inv2, o[1] * inv2), pack_bf16(o[2] * inv2, o[3] * inv2),
-                                                                            pack_bf16(o[4] * inv2, o[5] * inv2), pack_bf16(o[6] * inv2, o[7] * inv2));
+                        if (row < rows) {
+#pragma unroll
+                            for (int i = 0; i < 64; i += 8)
+                                *reinterpret_cast<uint4*>(dst + d + i) =
+                                    make_uint4(pack_bf16(o[i] * inv2, o[i + 1] * inv2), pack_bf16(o[i + 2] * inv2, o[i + 3] * inv2),
+                                               pack_bf16(o[i + 4] * inv2, o[i + 5] * inv2), pack_bf16(o[i + 6] * inv2, o[i + 7] * inv2));
+                        }
                     }
                 }
                 half_barrier(w);   // (s_last)
@@ -341,16 +444,17 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
         }
     } else if (warp < 12) {
         // ---------------- 4-bit tiles to f16 operands ----------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
         const int g = lane >> 2, t = lane & 3, wq = warp - 8;
         int n = 0;   // tiles so far: stage n & 1, its use n >> 1
-        for (; it.next(a, G); it.done()) {
-            const int tile0 = it.range.lo / PF_TILE, h = it.h;
+        for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
+            const PrefillItem& it = *item;
+            const int tile0 = it.tile0, h = it.h, k_end = it.k1;
             const int32_t* trow = a.table + (long long)it.b * a.cols;
-            const int blk_hi = (it.range.hi + 15) >> 4;
+            const int blk_hi = (it.hi + 15) >> 4;
             auto page_of = [&](int k) {   // lane i: block i & 1 of this warp in tile k + i / 2
                 const int kb = (tile0 + k + (lane >> 1)) * (PF_TILE / 16) + wq * 2 + (lane & 1);
-                return kb < blk_hi && k + (lane >> 1) < it.k1 ? trow[kb / P16] : -1;
+                return kb < blk_hi && k + (lane >> 1) < k_end ? trow[kb / P16] : -1;
             };
             auto block_at = [&](int id, int k, int which) -> const uint8_t* {
                 if (id < 0 || id >= a.cache.pages) return nullptr;
@@ -368,7 +472,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) load_v<D>(vr[i], blk[i], lane);
-            for (int k = it.k0; k < it.k1; k++, n++) {
+            for (int k = it.k0; k < k_end; k++, n++) {
                 const int st = n & 1;
                 const uint32_t ph = ((uint32_t)(n >> 1) & 1u) ^ 1u;
                 wait(k_empty(st), ph);
@@ -401,7 +505,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_full(st));
-                if (k + 1 < it.k1) {
+                if (k + 1 < k_end) {
                     if (k + 1 - ids_at == 16) {
                         ids_at = k + 1;
                         ids = page_of(ids_at);
@@ -440,14 +544,14 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_full(st));
-                if (k + 1 < it.k1) {
+                if (k + 1 < k_end) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) load_v<D>(vr[i], blk[i], lane);
                 }
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
         if (warp == 12) {
             // ---------------- MMA issue (the whole warp walks the loop, one lane issues) ----------------
             const bool leader = elect_one();
@@ -464,15 +568,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                         tc_mma<KIND_BF16, 1>(tmem + C::S_COL + 128u * w, da + 2u * j, db + 2u * j, idesc_s, pd + j > 0 ? 1u : 0u, 0, 0);
                 }
             };
-            auto product_o = [&](int w, int st, bool fresh) {
+            auto product_o = [&](int w, int st, int j0, bool fresh) {
                 const uint64_t db = smem_desc_v(base + C::OFF_V + (uint32_t)st * C::KV_BYTES, C::PANEL);
 #pragma unroll
-                for (int j = 0; j < 8; j++)   // sixteen tokens each
-                    tc_mma_f16_ts(tmem + C::O_COL + (uint32_t)D * w, tmem + C::S_COL + 128u * w + 8u * j, db + 128u * j, idesc_o,
-                                  fresh && j == 0 ? 0u : 1u);
+                for (int j = j0; j < j0 + 4; j++)   // sixteen tokens each
+                    tc_mma_f16_ts(tmem + C::O_COL + (uint32_t)D * w, tmem + C::S_COL + C::P_COL + 128u * w + 8u * j, db + 128u * j, idesc_o,
+                                  fresh && j == j0 ? 0u : 1u);
             };
-            for (; it.next(a, G); it.done()) {
-                const int halves = it.r.n * G - it.rt * PF_ROWS > 128 ? 2 : 1;
+            for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
+                const PrefillItem& it = *item;
+                const int halves = it.rows > 128 ? 2 : 1;
                 const int count = it.k1 - it.k0;
                 wait(k_full(n & 1), (uint32_t)(n >> 1) & 1u);
                 for (int w = 0; w < halves; w++) {
@@ -490,16 +595,19 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     const bool more = i + 1 < count;
                     wait(v_full(st), (uint32_t)(n >> 1) & 1u);
                     for (int w = 0; w < halves; w++) {
-                        wait(p_full(w), ph_p[w]);
-                        ph_p[w] ^= 1u;
+                        wait(p_half(w), ph_p[w]);
                         if (i == 0) {
                             wait(o_empty(w), (items[w] & 1u) ^ 1u);
                             items[w]++;
                         }
+                        tc_fence_after();
+                        if (leader) product_o(w, st, 4, i == 0);
                         if (w == 0 && more) wait(k_full(nx), (uint32_t)((n + 1) >> 1) & 1u);
+                        wait(p_full(w), ph_p[w]);
+                        ph_p[w] ^= 1u;
                         tc_fence_after();
                         if (leader) {
-                            product_o(w, st, i == 0);
+                            product_o(w, st, 0, false);
                             if (w == halves - 1) tc_commit(v_empty(st));
                             if (more) {
                                 product_s(w, nx);
@@ -514,6 +622,37 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             }
             if (leader) tc_commit(drained);   // nothing of this block is in flight when tensor memory is freed
             wait(drained, 0);
+        } else if (warp == 13) {
+            // ---------------- the items, a few ahead ----------------
+            Items<PF_ROWS, PF_TILE> items(a, G, run);
+            for (int no = 0;; no++) {
+                const int i = no % C::RING;
+                wait(item_empty(i), ((uint32_t)(no / C::RING) & 1u) ^ 1u);
+                const bool more = items.more() && !*wait.dead;
+                if (lane == 0) {
+                    PrefillItem x{};
+                    if (more) {
+                        x.k0 = items.k0;
+                        x.k1 = items.k1;
+                        x.tile0 = items.range.lo / PF_TILE;
+                        x.hi = items.range.hi;
+                        x.b = items.b;
+                        x.h = items.h;
+                        x.row0 = items.r.row0;
+                        x.first = items.rt * PF_ROWS;
+                        x.rows = min(PF_ROWS, items.r.n * G - x.first);
+                        x.n = items.r.n;
+                        x.kv_len = items.r.kv_len;
+                        x.c_first = items.whole() ? 0 : items.first_block();
+                        x.c_last = items.whole() ? 0 : items.last_block();
+                    }
+                    s_items[i] = x;
+                    mbar_arrive(item_full(i));
+                }
+                __syncwarp();
+                if (!more) break;
+                items.next(a, G);
+            }
         }
     }
     tc_fence_before();
