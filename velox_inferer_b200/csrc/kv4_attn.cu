@@ -119,7 +119,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ long long s_red[WARPS], s_found[2];
     __shared__ int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int hkv = a.cache.kv_heads, G = a.heads / hkv, P16 = a.cache.page_size >> 4;
+    const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = __ffs(a.cache.page_size) - 5;   // (blocks per page: a power of two)
     if (tid == 0) grid_launch_dependents();
     grid_dependency_wait();
 
@@ -204,12 +204,12 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
         const int blk_hi = (range.hi + 15) >> 4;
         auto page_of = [&](int k) {
             const int kb = (tile0 + k + (lane >> 1)) * (TILE / 16) + warp * 2 + (lane & 1);
-            return kb < blk_hi ? trow[kb / P16] : -1;
+            return kb < blk_hi ? trow[kb >> page_shift] : -1;
         };
         auto block_at = [&](int id, int k, int which) -> const uint8_t* {
             if (id < 0 || id >= a.cache.pages) return nullptr;
             const int kb = (tile0 + k) * (TILE / 16) + warp * 2 + which;
-            return a.cache.blocks + (((long long)id * hkv + h) * P16 + kb % P16) * (18 * D);
+            return a.cache.blocks + ((((long long)id * hkv + h) << page_shift) + (kb & ((1 << page_shift) - 1))) * (18 * D);
         };
         int ids = page_of(k0), ids_at = k0;
         const uint8_t* blk[2];

@@ -84,6 +84,18 @@ __device__ __forceinline__ uint64_t smem_desc_v(uint32_t addr, uint32_t panel) {
     return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// 2^x in multiplications and additions: x = j + f, j whole, |f| <= 1/2; a polynomial of degree 4 in f (minimax fit,
+// relative error 2.6e-6), j added to its exponent. x below -126 gives 2^-126.
+__device__ __forceinline__ float exp2_fma(float x) {
+    x = fmaxf(x, -126.0f);
+    const float r = x + 12582912.0f;   // 1.5 * 2^23: the sum's last bits are j
+    const float f = x - (r - 12582912.0f);
+    float p = fmaf(9.5701022e-3f, f, 5.5917859e-2f);
+    p = fmaf(p, f, 0.24024744f);
+    p = fmaf(p, f, 0.69312179f);
+    p = fmaf(p, f, 0.99999928f);
+    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -125,7 +137,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ int s_last[2];
     __shared__ PrefillItem s_items[C::RING];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int hkv = a.cache.kv_heads, G = a.heads / hkv, P16 = a.cache.page_size >> 4;
+    const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = __ffs(a.cache.page_size) - 5;   // (blocks per page: a power of two)
     const uint32_t bars = base + C::OFF_BARS;
     auto k_full = [&](int s) { return bars + 8u * s; };
     auto k_empty = [&](int s) { return bars + 16u + 8u * s; };
@@ -252,7 +264,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             // Which of the next four tiles' 32 blocks lie in the cache: the ids are read four tiles ahead.
             auto page_id = [&](int k) {
                 const int kb = (tile0 + k) * (PF_TILE / 16) + lane;
-                return kb < blk_hi ? trow[kb / P16] : -1;
+                return kb < blk_hi ? trow[kb >> page_shift] : -1;
             };
             int ids = page_id(it.k0);
             uint32_t there4 = 0;
@@ -267,18 +279,27 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 wait(s_full(w), ph_s);
                 ph_s ^= 1u;
                 tc_fence_after();
+                const int tok = (tile0 + k) * PF_TILE;
+                if (tok < all_lo || tok + PF_TILE > all_hi || there != 0xffu) {
+                    // A tile with masked tokens: masked in place, in a loop of its own, so that the code that every
+                    // tile runs through stays short (instruction fetch is what this loop waits for most).
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t s[32];
+                        tc_ld32(ts + 32u * c, s);
+                        tc_wait_ld_of(s);
+                        const int lo = lim_lo - tok - c * 32, hi = lim_hi - tok - c * 32;
+                        const uint32_t two = there >> (c * 2);
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (i < lo || i >= hi || !(two >> (i / 16) & 1u)) s[i] = __float_as_uint(-INFINITY);
+                        tc_st32(ts + 32u * c, s);
+                    }
+                    tc_wait_st();
+                }
                 // Scores in four chunks of 32 columns: 0 and 1 are read for the maximum and once more for the
                 // exponentials, 2 and 3 stay in registers in between. (All 128 at once spill, and with nearly
                 // all of the L1 given to operands a spilled register comes back from L2.)
-                const int tok = (tile0 + k) * PF_TILE;
-                const bool edge = tok < all_lo || tok + PF_TILE > all_hi || there != 0xffu;
-                auto mask = [&](uint32_t (&s)[32], int c) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const int j = tok + c * 32 + i;
-                        if (j < lim_lo || j >= lim_hi || !(there >> (c * 2 + i / 16) & 1u)) s[i] = __float_as_uint(-INFINITY);
-                    }
-                };
                 auto max32 = [&](const uint32_t (&s)[32]) {
                     float u = __uint_as_float(s[0]), v = __uint_as_float(s[1]);
 #pragma unroll
@@ -295,16 +316,10 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 tc_wait_ld_of(x0);
                 tc_wait_ld_of(x1);
                 tc_wait_ld_of(x2);
-                if (edge) {
-                    mask(x0, 0);
-                    mask(x1, 1);
-                    mask(x2, 2);
-                }
                 float mx = fmaxf(max32(x0), max32(x1));
                 tc_ld32(ts + 96u, x1);
                 mx = fmaxf(mx, max32(x2));
                 tc_wait_ld_of(x1);
-                if (edge) mask(x1, 3);
                 mx = fmaxf(mx, max32(x1));
                 mx *= ksc;
                 if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
@@ -331,8 +346,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float x = exp2_approx(fmaf(__uint_as_float(s[2 * i]), ksc, off));
-                        const float y = exp2_approx(fmaf(__uint_as_float(s[2 * i + 1]), ksc, off));
+                        float x = fmaf(__uint_as_float(s[2 * i]), ksc, off), y = fmaf(__uint_as_float(s[2 * i + 1]), ksc, off);
+                        x = exp2_approx(x);
+                        y = exp2_approx(y);
                         l0 += x;
                         l1 += y;
                         p[i] = pack_f16(x, y);
@@ -348,10 +364,6 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 tc_ld32(ts + 32u, x1);
                 tc_wait_ld_of(x0);
                 tc_wait_ld_of(x1);
-                if (edge) {
-                    mask(x0, 0);
-                    mask(x1, 1);
-                }
                 chunk(x0, 0);
                 chunk(x1, 1);
                 l += l0 + l1;
@@ -454,12 +466,12 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             const int blk_hi = (it.hi + 15) >> 4;
             auto page_of = [&](int k) {   // lane i: block i & 1 of this warp in tile k + i / 2
                 const int kb = (tile0 + k + (lane >> 1)) * (PF_TILE / 16) + wq * 2 + (lane & 1);
-                return kb < blk_hi && k + (lane >> 1) < k_end ? trow[kb / P16] : -1;
+                return kb < blk_hi && k + (lane >> 1) < k_end ? trow[kb >> page_shift] : -1;
             };
             auto block_at = [&](int id, int k, int which) -> const uint8_t* {
                 if (id < 0 || id >= a.cache.pages) return nullptr;
                 const int kb = (tile0 + k) * (PF_TILE / 16) + wq * 2 + which;
-                return a.cache.blocks + (((long long)id * hkv + h) * P16 + kb % P16) * (18 * D);
+                return a.cache.blocks + ((((long long)id * hkv + h) << page_shift) + (kb & ((1 << page_shift) - 1))) * (18 * D);
             };
             int ids = page_of(it.k0), ids_at = it.k0;
             const uint8_t* blk[2];
