@@ -327,7 +327,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     m = v;
                     l *= f;
                     if (k > it.k0) {   // (the first tile's product overwrites O)
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
                             tc_ld32(to + 32u * c, o);
@@ -355,17 +355,20 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     }
                     tc_st16(ts + C::P_COL + 16u * c, p);
                 };
-                tc_ld32(ts, x0);
-                chunk(x2, 2);
-                chunk(x1, 3);
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(p_half(w));
-                tc_ld32(ts + 32u, x1);
-                tc_wait_ld_of(x0);
-                tc_wait_ld_of(x1);
-                chunk(x0, 0);
-                chunk(x1, 1);
+#pragma unroll 1
+                for (int c = 2; c >= 0; c -= 2) {
+                    chunk(x2, c);
+                    chunk(x1, c + 1);
+                    if (c > 0) {
+                        tc_ld32(ts, x2);
+                        tc_ld32(ts + 32u, x1);
+                        tc_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(p_half(w));
+                        tc_wait_ld_of(x2);
+                        tc_wait_ld_of(x1);
+                    }
+                }
                 l += l0 + l1;
                 tc_wait_st();
                 tc_fence_before();
