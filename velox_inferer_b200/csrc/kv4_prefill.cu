@@ -50,20 +50,22 @@ struct PrefillCfg {
 struct Waiter {
     volatile int* dead;
     __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) const {
-        if (mbar_try_wait(bar, parity)) return;
-        const unsigned long long t0 = global_timer_ns();
-        for (uint32_t spins = 1;; spins++) {
-            if (mbar_try_wait(bar, parity)) return;
-            if ((spins & 63u) == 0) {
-                if (*dead) return;
+        if (!mbar_try_wait(bar, parity)) {
+            const unsigned long long t0 = global_timer_ns();
+            for (uint32_t spins = 1; !mbar_try_wait(bar, parity); spins++) {
+                if ((spins & 63u) != 0) continue;
+                if (*dead) break;
                 if (global_timer_ns() - t0 > 2000000000ull) {
                     *dead = 1;
                     atomicExch(&g_kv4_status, KV4_TIMEOUT);
-                    return;
+                    break;
                 }
             }
         }
+        __syncwarp();   // lanes leave the poll one by one; what follows may be a collective of the whole warp
     }
+    // The same answer in every lane.
+    __device__ __forceinline__ bool given_up() const { return __any_sync(0xffffffffu, *dead != 0); }
 };
 
 // D[128 x N] (+)= A . B, f16 operands, f32 accumulator; A from tensor memory.
@@ -84,17 +86,16 @@ __device__ __forceinline__ uint64_t smem_desc_v(uint32_t addr, uint32_t panel) {
     return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// 2^x in multiplications and additions: x = j + f, j whole, |f| <= 1/2; a polynomial of degree 4 in f (minimax fit,
-// relative error 2.6e-6), j added to its exponent. x below -126 gives 2^-126.
-__device__ __forceinline__ float exp2_fma(float x) {
-    x = fmaxf(x, -126.0f);
-    const float r = x + 12582912.0f;   // 1.5 * 2^23: the sum's last bits are j
-    const float f = x - (r - 12582912.0f);
-    float p = fmaf(9.5701022e-3f, f, 5.5917859e-2f);
-    p = fmaf(p, f, 0.24024744f);
-    p = fmaf(p, f, 0.69312179f);
-    p = fmaf(p, f, 0.99999928f);
-    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
+// Two single-precision operations in one instruction.
+__device__ __forceinline__ void fma2(float& x, float& y, float m, float c) {
+    asm("{\n\t.reg .b64 v, m2, c2;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m2, {%2, %2};\n\tmov.b64 c2, {%3, %3};\n\t"
+        "fma.rn.f32x2 v, v, m2, c2;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float u, float v) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+        "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(u), "f"(v));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -113,7 +114,6 @@ __device__ __forceinline__ void tc_wait_ld_of(uint32_t (&r)[32]) {
                  : "memory");
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void half_barrier(int w) { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); }
 
 // An item as the roles see it.
 struct PrefillItem {
@@ -149,6 +149,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     auto o_full = [&](int w) { return bars + 112u + 8u * w; };
     auto o_empty = [&](int w) { return bars + 128u + 8u * w; };
     const uint32_t drained = bars + 144u;
+    auto joined = [&](int w) { return bars + 232u + 8u * w; };   // the threads of a half among themselves
     auto p_half = [&](int w) { return bars + 216u + 8u * w; };   // the last 64 tokens of P
     auto item_full = [&](int i) { return bars + 152u + 8u * i; };
     auto item_empty = [&](int i) { return bars + 184u + 8u * i; };
@@ -163,6 +164,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             mbar_init(v_empty(i), 1);
             mbar_init(q_full(i), 128);
             mbar_init(s_full(i), 1);
+            mbar_init(joined(i), 128);
             mbar_init(p_half(i), 128);
             mbar_init(p_full(i), 128);
             mbar_init(o_full(i), 1);
@@ -193,7 +195,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     auto take = [&]() -> const PrefillItem* {
         const int i = item_no % C::RING;
         wait(item_full(i), (uint32_t)(item_no / C::RING) & 1u);
-        return s_items[i].k1 > 0 && !*wait.dead ? &s_items[i] : nullptr;
+        return s_items[i].k1 > 0 && !wait.given_up() ? &s_items[i] : nullptr;
     };
     auto give_back = [&]() {
         __syncwarp();
@@ -203,14 +205,19 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
     if (warp < 8) {
         // ---------------- softmax of one half: a row per thread ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;" ::: "memory");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;" ::: "memory");
         const int w = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
         const uint32_t ts = tmem + lanes + C::S_COL + 128u * w, to = tmem + lanes + C::O_COL + (uint32_t)D * w;
         const float soft = score_factor(a);
         uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws + a.prefill_tickets);
         float* parts = reinterpret_cast<float*>(a.ws + a.prefill_parts);
-        uint32_t ph_s = 0, ph_o = 0;
+        uint32_t ph_s = 0, ph_o = 0, ph_j = 0;
+        auto half_barrier = [&]() {   // of the half's 128 threads, and bounded like every wait here
+            mbar_arrive(joined(w));
+            wait(joined(w), ph_j);
+            ph_j ^= 1u;
+        };
         for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
             const PrefillItem& it = *item;
             const int rows = it.rows - 128 * w;   // of this half
@@ -346,11 +353,11 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        float x = fmaf(__uint_as_float(s[2 * i]), ksc, off), y = fmaf(__uint_as_float(s[2 * i + 1]), ksc, off);
+                        float x = __uint_as_float(s[2 * i]), y = __uint_as_float(s[2 * i + 1]);
+                        fma2(x, y, ksc, off);
                         x = exp2_approx(x);
                         y = exp2_approx(y);
-                        l0 += x;
-                        l1 += y;
+                        add2(l0, l1, x, y);
                         p[i] = pack_f16(x, y);
                     }
                     tc_st16(ts + C::P_COL + 16u * c, p);
@@ -413,9 +420,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 part[row] = m;
                 part[128 + row] = l;
                 __threadfence();
-                half_barrier(w);
+                half_barrier();
                 if (row == 0) s_last[w] = atomicAdd(&tickets[c_first * 2 + w], 1u) == (uint32_t)(c_last - c_first);
-                half_barrier(w);
+                half_barrier();
                 if (s_last[w]) {   // the half's last block: join the parts in token order
                     __threadfence();
                     if (row == 0) tickets[c_first * 2 + w] = 0;
@@ -454,12 +461,12 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                         }
                     }
                 }
-                half_barrier(w);   // (s_last)
+                half_barrier();   // (s_last)
             }
         }
     } else if (warp < 12) {
         // ---------------- 4-bit tiles to f16 operands ----------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;" ::: "memory");
         const int g = lane >> 2, t = lane & 3, wq = warp - 8;
         int n = 0;   // tiles so far: stage n & 1, its use n >> 1
         for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
@@ -566,7 +573,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;" ::: "memory");
         if (warp == 12) {
             // ---------------- MMA issue (the whole warp walks the loop, one lane issues) ----------------
             const bool leader = elect_one();
@@ -643,7 +650,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int no = 0;; no++) {
                 const int i = no % C::RING;
                 wait(item_empty(i), ((uint32_t)(no / C::RING) & 1u) ^ 1u);
-                const bool more = items.more() && !*wait.dead;
+                const bool more = items.more() && !wait.given_up();
                 if (lane == 0) {
                     PrefillItem x{};
                     if (more) {
