@@ -205,7 +205,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
     if (warp < 8) {
         // ---------------- softmax of one half: a row per thread ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;" ::: "memory");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;" ::: "memory");
         const int w = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16;
         const uint32_t ts = tmem + lanes + C::S_COL + 128u * w, to = tmem + lanes + C::O_COL + (uint32_t)D * w;
@@ -466,7 +466,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
         }
     } else if (warp < 12) {
         // ---------------- 4-bit tiles to f16 operands ----------------
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;" ::: "memory");
         const int g = lane >> 2, t = lane & 3, wq = warp - 8;
         int n = 0;   // tiles so far: stage n & 1, its use n >> 1
         for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
@@ -573,7 +573,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;" ::: "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
         if (warp == 12) {
             // ---------------- MMA issue (the whole warp walks the loop, one lane issues) ----------------
             const bool leader = elect_one();
