@@ -164,8 +164,11 @@ int kv4_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t*
 // ---- norms, rotation, quantised store ------------------------------------------------------------
 //
 // A row (one head of one token) is held by D/8 lanes, eight consecutive values each; a warp takes
-// 32 / (D/8) rows at once and ROWS of those row groups of one token, so the token's cosines and
-// sines are loaded once for all of them and every row's loads are in flight together.
+// 32 / (D/8) rows at once. A task is ROWS such groups of q rows of one token, or as many of its k and v rows, so
+// the token's cosines and sines are loaded once per task. Warps walk the tasks with the grid's stride, all q tasks
+// first, and request the next task's rows before they finish this one's. With one task per warp the pass waited
+// for three memory round trips per 2 KB (2048 tokens of 64 + 8 + 8 heads, bf16: 73 us); with q, k and v rows mixed
+// in a task the warps that met the k rows (f64) every time ended last (75 us); XXX us now.
 //   q: x / sqrt(mean(x^2) + eps) * (offset + w), rotated; f32 throughout, rounded once.
 //   k on its way into the cache: the same in f64. A 4-bit code changes by a whole step when the value
 //   before it crosses a border, so the value handed to the quantiser is the correctly rounded f32 of
@@ -173,70 +176,18 @@ int kv4_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t*
 //   The quantiser is the library's (actquant.cu): s = e4m3(divisor * amax / 6), code =
 //   e2m1(x * divisor / s), single-precision steps.
 
-template <typename T>
-__device__ __forceinline__ T rope_sqrt_inv(T mean_eps);
-template <>
-__device__ __forceinline__ float rope_sqrt_inv<float>(float v) { return __fdiv_rn(1.0f, __fsqrt_rn(v)); }
-template <>
-__device__ __forceinline__ double rope_sqrt_inv<double>(double v) { return 1.0 / sqrt(v); }
-
-// Norm and rotation of a row's eight values in this lane, in T.
-template <typename T, int LPR>
-__device__ __forceinline__ void norm_rotate(T (&x)[8], const float* __restrict__ weight, int offset, float eps,
-                                            const float (&cs)[16], int rot, int interleaved, int li, bool rotate) {
-    constexpr int D = LPR * 8;
-    if (weight) {
-        T ss = 0;
+__device__ __forceinline__ void unpack8(const uint4& a, float (&x)[8]) {
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const T inv = rope_sqrt_inv<T>(ss / (T)D + (T)eps);
-        const float4 w0 = *reinterpret_cast<const float4*>(weight + li * 8);
-        const float4 w1 = *reinterpret_cast<const float4*>(weight + li * 8 + 4);
-        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = x[i] * inv * (offset ? (T)1 + (T)w[i] : (T)w[i]);
-    }
-    if (!rotate) return;   // uniform over the warp
-    const bool mine = li * 8 < rot;
-    if (interleaved) {
-        if (mine) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const T c = (T)cs[i], s = (T)cs[8 + i], a = x[2 * i], b = x[2 * i + 1];
-                x[2 * i] = a * c - b * s;
-                x[2 * i + 1] = b * c + a * s;
-            }
-        }
-    } else {
-        const int half_lanes = rot / 16;
-        const bool first = li < half_lanes;
-        const int partner = (threadIdx.x & 31) + (mine ? (first ? half_lanes : -half_lanes) : 0);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const T o = __shfl_sync(0xffffffffu, x[i], partner);
-            const T c = (T)cs[i], s = (T)cs[8 + i];
-            if (mine) x[i] = first ? x[i] * c - o * s : x[i] * c + o * s;
-        }
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
 }
-
-__device__ __forceinline__ void load_row8(const void* p, long long at, int f32, float (&x)[8]) {
-    if (f32) {
-        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at);
-        const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at);
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void unpack8(const uint4& a, const uint4& b, float (&x)[8]) {
+    const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(u[i] << 16);
-            x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-        }
-    }
+    for (int i = 0; i < 8; i++) x[i] = __uint_as_float(u[i]);
 }
 
 __device__ __forceinline__ void store_row8(void* p, long long at, int f32, const float (&x)[8]) {
@@ -255,6 +206,88 @@ __device__ __forceinline__ void store_row8(void* p, long long at, int f32, const
     }
 }
 
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// What a lane needs of the rotation of its eight dimensions: y = c x + s (its partner's x), with the sign in s. Pairs
+// of neighbours are in the lane itself (the first four entries); a lane that is not rotated has c = 1, s = 0 and
+// itself as the partner.
+struct Turn {
+    float c[8], s[8];
+    int partner;
+};
+
+template <typename T>
+__device__ __forceinline__ void rotate8(T (&x)[8], const Turn& t, int interleaved) {
+    if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const T a = x[2 * i], b = x[2 * i + 1], c = (T)t.c[i], s = (T)t.s[i];
+            x[2 * i] = a * c - b * s;
+            x[2 * i + 1] = b * c + a * s;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const T o = __shfl_sync(0xffffffffu, x[i], t.partner);
+            x[i] = x[i] * (T)t.c[i] + o * (T)t.s[i];
+        }
+    }
+}
+
+template <int LPR>
+__device__ __forceinline__ void norm8_f32(float (&x)[8], const float* __restrict__ weight, int offset, float eps, int li) {
+    constexpr int D = LPR * 8;
+    float w[8];
+    load8(weight + li * 8, w);
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss * (1.0f / D) + eps);   // (two units in the last place at most)
+    const float one = offset ? 1.0f : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = x[i] * inv * (one + w[i]);
+}
+
+// The same in f64. 1 / sqrt by two Newton steps from the single-precision estimate (2^-22 -> 2^-44 -> 2^-88): a
+// few units of 2^-53.
+template <int LPR>
+__device__ __forceinline__ void norm8_f64(double (&x)[8], const float* __restrict__ weight, int offset, float eps, int li) {
+    constexpr int D = LPR * 8;
+    float w[8];
+    load8(weight + li * 8, w);
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) ss = fma(x[i], x[i], ss);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const double v = ss * (1.0 / D) + (double)eps;
+    double inv;
+    // (estimates outside f32's range, for sums that a norm never sees in earnest, take the plain route)
+    if (v > 1e-30 && v < 1e30) {
+        inv = (double)rsqrtf((float)v);
+#pragma unroll
+        for (int i = 0; i < 2; i++) inv = inv * fma(-0.5 * v * inv, inv, 1.5);
+    } else {
+        inv = 1.0 / sqrt(v);
+    }
+    const double one = offset ? 1.0 : 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = x[i] * inv * (one + (double)w[i]);
+}
+
+// a / b for normal quotients from r = 1 / b: one correction of the rounded product gives the correctly
+// rounded quotient.
+__device__ __forceinline__ float quotient(float a, float b, float r) {
+    const float q = a * r;
+    return fmaf(fmaf(-q, b, a), r, q);
+}
+
 // Quantises this lane's eight values (two neighbouring lanes make a group of 16).
 __device__ __forceinline__ uint32_t quant8(const float (&x)[8], float divisor, uint32_t& scale) {
     float amax = 0.0f;
@@ -264,170 +297,217 @@ __device__ __forceinline__ uint32_t quant8(const float (&x)[8], float divisor, u
     scale = f32_to_e4m3(__fdiv_rn(__fmul_rn(divisor, amax), 6.0f));
     uint32_t codes = 0;
     if (scale != 0) {
-        const float ds = e4m3_to_f32(scale);
+        const float ds = e4m3_to_f32(scale), r = __fdiv_rn(1.0f, ds);
+        float q[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            codes |= f32x2_to_e2m1x2(__fdiv_rn(__fmul_rn(x[2 * i], divisor), ds),
-                                     __fdiv_rn(__fmul_rn(x[2 * i + 1], divisor), ds)) << (8 * i);
+        for (int i = 0; i < 8; i++)   // (past 1e30 a value saturates at any scale; kept finite for the correction)
+            q[i] = quotient(fminf(fmaxf(__fmul_rn(x[i], divisor), -1e30f), 1e30f), ds, r);
+#pragma unroll
+        for (int i = 0; i < 4; i++) codes |= f32x2_to_e2m1x2(q[2 * i], q[2 * i + 1]) << (8 * i);
     }
     return codes;
 }
 
 constexpr int ROPE_T = 128;
+// Row groups per task once there is work for every warp, and blocks per SM that this leaves room for.
+constexpr int rope_rows(bool f32) { return f32 ? 2 : 4; }
+constexpr int rope_blocks(int rows) { return rows == 1 ? 8 : 5; }
 
-template <int LPR, int ROWS>
-__global__ void __launch_bounds__(ROPE_T)
-kv4_norm_rope_kernel(Kv4RopeArgs a) {
+template <int LPR, int ROWS, bool F32>
+__global__ void __launch_bounds__(ROPE_T, rope_blocks(ROWS))
+kv4_norm_rope_kernel(const __grid_constant__ Kv4RopeArgs a) {
     constexpr int D = LPR * 8, RPG = 32 / LPR;   // rows per group
     const int lane = threadIdx.x & 31, li = lane % LPR, sub = lane / LPR;
     if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
-    const int gq = (a.heads + RPG - 1) / RPG, gk = (a.kv_heads + RPG - 1) / RPG;
-    const int groups = gq + gk + (a.store ? gk : 0);
-    const int chunks = (groups + ROWS - 1) / ROWS;
-    const long long task = (long long)blockIdx.x * (ROPE_T / 32) + (threadIdx.x >> 5);
-    if (task >= (long long)a.tokens * chunks) return;
-    const long long tok = task / chunks;
-    const int g0 = (int)(task - tok * chunks) * ROWS;
-    const int pos = a.positions ? a.positions[tok] : 0;
-    const int slot = a.store ? a.slots[tok] : 0;
+    // Tasks of a token: cq of q rows, then ck of k rows, or of k and v rows in turn where they are stored.
+    const unsigned gq = (a.heads + RPG - 1) / RPG, gk = (a.kv_heads + RPG - 1) / RPG * (a.store ? 2 : 1);
+    const unsigned cq = (gq + ROWS - 1) / ROWS, ck = (gk + ROWS - 1) / ROWS;
+    const unsigned tq = (unsigned)a.tokens * cq, total = tq + (unsigned)a.tokens * ck, stride = gridDim.x * (ROPE_T / 32);
     const long long slots = a.store ? a.cache.pages * a.cache.page_size : 0;
-    // a row behind the last sequence, or outside the table: left as it was
-    const bool live = pos >= 0 && (a.rope == nullptr || pos < a.rope_len);
-    if (!live) return;
-    const bool keep = a.store && slot >= 0 && slot < slots;
 
-    float x[ROWS][8];
+    struct Task {
+        uint4 x[ROWS][F32 ? 2 : 1];
+        int pos, slot;
+        unsigned tok, g0;
+    };
+    // Group g of a token's k / v rows: the k and the v row of a head group follow each other.
+    auto head_of = [&](bool q, unsigned g) { return (int)(q || !a.store ? g : g >> 1) * RPG + sub; };
+    auto fetch = [&](unsigned task, Task& t) {
+        const bool q = task < tq;
+        if (!q) task -= tq;
+        t.tok = task / (q ? cq : ck);
+        t.g0 = (task - t.tok * (q ? cq : ck)) * ROWS;
+        t.pos = a.positions ? a.positions[t.tok] : 0;
+        t.slot = a.store ? a.slots[t.tok] : 0;
 #pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-        const int g = g0 + r;
-        const int kind = g < gq ? 0 : (g < gq + gk ? 1 : 2);
-        const int head = (g - (kind == 0 ? 0 : kind == 1 ? gq : gq + gk)) * RPG + sub;
-        const bool on = g < groups && head < (kind == 0 ? a.heads : a.kv_heads);
-        if (on) {
-            const void* p = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-            const long long st = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
-            load_row8(p, tok * st + head * D + li * 8, a.in_f32, x[r]);
-        } else {
+        for (int r = 0; r < ROWS; r++) {
+            const unsigned g = t.g0 + r;
+            const bool v = !q && a.store && (g & 1);
+            const int head = head_of(q, g);
+            if (head < (q ? a.heads : a.kv_heads)) {
+                const void* p = q ? a.q : v ? a.v : a.k;
+                const long long at = (long long)t.tok * (q ? a.q_stride : v ? a.v_stride : a.k_stride) + head * D + li * 8;
+                const uint4* src = F32 ? reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at)
+                                       : reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[r][i] = 0.0f;
-        }
-    }
-    float cs[16] = {};
-    if (a.rope && li * 8 < a.rot) {
-        const float* row = a.rope + (long long)pos * a.rot;
-        if (a.interleaved) {   // four pairs
-            const float4 c = *reinterpret_cast<const float4*>(row + li * 4);
-            const float4 s = *reinterpret_cast<const float4*>(row + a.rot / 2 + li * 4);
-            cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
-            cs[8] = s.x; cs[9] = s.y; cs[10] = s.z; cs[11] = s.w;
-        } else {
-            const int at = li * 8 % (a.rot / 2);
+                for (int i = 0; i < (F32 ? 2 : 1); i++) t.x[r][i] = src[i];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float4 c = *reinterpret_cast<const float4*>(row + at + 4 * i);
-                const float4 s = *reinterpret_cast<const float4*>(row + a.rot / 2 + at + 4 * i);
-                cs[4 * i] = c.x; cs[4 * i + 1] = c.y; cs[4 * i + 2] = c.z; cs[4 * i + 3] = c.w;
-                cs[8 + 4 * i] = s.x; cs[9 + 4 * i] = s.y; cs[10 + 4 * i] = s.z; cs[11 + 4 * i] = s.w;
+                for (int i = 0; i < (F32 ? 2 : 1); i++) t.x[r][i] = make_uint4(0, 0, 0, 0);
             }
         }
-    }
+    };
+
+    unsigned task = blockIdx.x * (ROPE_T / 32) + (threadIdx.x >> 5);
+    if (task >= total) return;
+    Task next;
+    fetch(task, next);
+    for (bool more = true; more; task += stride) {
+        const Task t = next;
+        more = total - task > stride;
+        // a row behind the last sequence, or outside the table: left as it was
+        const bool live = t.pos >= 0 && (a.rope == nullptr || t.pos < a.rope_len);
+        Turn turn;
+        turn.partner = lane;
 #pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-        const int g = g0 + r;   // uniform over the warp
-        if (g >= groups) break;
-        const int kind = g < gq ? 0 : (g < gq + gk ? 1 : 2);
-        const int head = (g - (kind == 0 ? 0 : kind == 1 ? gq : gq + gk)) * RPG + sub;
-        const bool on = head < (kind == 0 ? a.heads : a.kv_heads);
-        if (kind == 0 || (kind == 1 && !a.store)) {
-            norm_rotate<float, LPR>(x[r], kind == 0 ? a.q_weight : a.k_weight, a.offset, a.eps, cs, a.rot, a.interleaved, li,
-                                    a.rope != nullptr);
-            if (on) store_row8(kind == 0 ? a.q_out : a.k_out, tok * (kind == 0 ? a.q_out_stride : a.k_out_stride) + head * D + li * 8,
-                               a.out_f32, x[r]);
-            continue;
+        for (int i = 0; i < 8; i++) {
+            turn.c[i] = 1.0f;
+            turn.s[i] = 0.0f;
         }
-        if (kind == 1 && (a.k_weight || a.rope)) {
-            double y[8];
+        if (a.rope && live && li * 8 < a.rot) {
+            const int half = a.rot / 2, half_lanes = a.rot / 16;
+            const float* row = a.rope + (long long)t.pos * a.rot;
+            if (a.interleaved) {   // four pairs
+                const float4 c = *reinterpret_cast<const float4*>(row + li * 4), s = *reinterpret_cast<const float4*>(row + half + li * 4);
+                turn.c[0] = c.x; turn.c[1] = c.y; turn.c[2] = c.z; turn.c[3] = c.w;
+                turn.s[0] = s.x; turn.s[1] = s.y; turn.s[2] = s.z; turn.s[3] = s.w;
+            } else {
+                const bool first = li < half_lanes;
+                turn.partner = lane + (first ? half_lanes : -half_lanes);
+                load8(row + (first ? li : li - half_lanes) * 8, turn.c);
+                load8(row + half + (first ? li : li - half_lanes) * 8, turn.s);
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = (double)x[r][i];
-            norm_rotate<double, LPR>(y, a.k_weight, a.offset, a.eps, cs, a.rot, a.interleaved, li, a.rope != nullptr);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[r][i] = (float)y[i];
+                for (int i = 0; i < 8; i++) turn.s[i] = first ? -turn.s[i] : turn.s[i];
+            }
         }
-        uint32_t scale;
-        const uint32_t codes = quant8(x[r], kind == 1 ? a.cache.k_div : a.cache.v_div, scale);
-        if (on && keep) {
-            int tau;
-            uint8_t* blk = kv4_block_of(a.cache, slot, head, tau);
-            // (eight values = four code bytes; a V piece of D/16 bytes holds two or one such words)
-            *reinterpret_cast<uint32_t*>(blk + (kind == 1 ? kv4_k_code(D, tau, li * 4) : kv4_v_code(D, tau, li * 4))) = codes;
-            if ((li & 1) == 0) blk[kind == 1 ? kv4_k_scale(D, tau, li >> 1) : kv4_v_scale(D, tau, li >> 1)] = (uint8_t)scale;
+        if (more) fetch(task + stride, next);
+        if (!live) continue;   // uniform over the warp
+        const bool q = task < tq;
+        if (q || !a.store) {
+            const float* weight = q ? a.q_weight : a.k_weight;
+            const int heads = q ? a.heads : a.kv_heads;
+            const long long at = (long long)t.tok * (q ? a.q_out_stride : a.k_out_stride) + li * 8;
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                const int head = (int)(t.g0 + r) * RPG + sub;
+                float x[8];
+                if (F32) unpack8(t.x[r][0], t.x[r][F32 ? 1 : 0], x); else unpack8(t.x[r][0], x);
+                if (weight) norm8_f32<LPR>(x, weight, a.offset, a.eps, li);
+                if (a.rope) rotate8(x, turn, a.interleaved);
+                if (head < heads) store_row8(q ? a.q_out : a.k_out, at + head * D, a.out_f32, x);
+            }
+        } else {
+            const bool keep = t.slot >= 0 && t.slot < slots;
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                const unsigned g = t.g0 + r;   // uniform over the warp
+                const int head = head_of(false, g);
+                const bool v = g & 1;
+                float x[8];
+                if (F32) unpack8(t.x[r][0], t.x[r][F32 ? 1 : 0], x); else unpack8(t.x[r][0], x);
+                if (!v && (a.k_weight || a.rope)) {
+                    double y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = (double)x[i];
+                    if (a.k_weight) norm8_f64<LPR>(y, a.k_weight, a.offset, a.eps, li);
+                    if (a.rope) rotate8(y, turn, a.interleaved);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = (float)y[i];
+                }
+                uint32_t scale;
+                const uint32_t codes = quant8(x, v ? a.cache.v_div : a.cache.k_div, scale);
+                if (head < a.kv_heads && keep) {
+                    int tau;
+                    uint8_t* blk = kv4_block_of(a.cache, t.slot, head, tau);
+                    // (eight values = four code bytes; a V piece of D/16 bytes holds two or one such words)
+                    *reinterpret_cast<uint32_t*>(blk + (v ? kv4_v_code(D, tau, li * 4) : kv4_k_code(D, tau, li * 4))) = codes;
+                    if ((li & 1) == 0) blk[v ? kv4_v_scale(D, tau, li >> 1) : kv4_k_scale(D, tau, li >> 1)] = (uint8_t)scale;
+                }
+            }
         }
     }
 }
 
 int kv4_norm_rope(const Kv4RopeArgs& a) {
     const int rpg = 256 / a.head_dim;
-    const int gq = (a.heads + rpg - 1) / rpg, gk = (a.kv_heads + rpg - 1) / rpg;
-    const int groups = gq + gk * (a.store ? 2 : 1);
-    // Several row groups per warp once there are enough warps to fill the machine without it (four
-    // blocks of four warps per SM).
-    const int rows = (long long)a.tokens * ((groups + 3) / 4) >= 16LL * kv4_sms() ? 4 : 1;
-    const long long warps = (long long)a.tokens * ((groups + rows - 1) / rows);
-    const long long blocks = (warps + ROPE_T / 32 - 1) / (ROPE_T / 32);
-    if (blocks > 0x7fffffffLL) return VELOX_ERR_UNSUPPORTED;
+    const long long gq = (a.heads + rpg - 1) / rpg, gk = (a.kv_heads + rpg - 1) / rpg * (a.store ? 2 : 1);
+    // Several row groups per task once there are enough tasks to fill the machine without it (four blocks of four
+    // warps per SM).
+    const int many = rope_rows(a.in_f32);
+    auto tasks = [&](int rows) { return (long long)a.tokens * ((gq + rows - 1) / rows + (gk + rows - 1) / rows); };
+    const int rows = tasks(many) >= 16LL * kv4_sms() ? many : 1;
+    if (tasks(rows) > 0x7fffffffLL) return VELOX_ERR_UNSUPPORTED;
+    const long long fit = (long long)rope_blocks(rows) * kv4_sms();
+    long long blocks = (tasks(rows) + ROPE_T / 32 - 1) / (ROPE_T / 32);
+    if (blocks > fit) blocks = fit;
     EarlyLaunch l((unsigned)blocks, ROPE_T);
-#define VX_ROPE(LPR)                                                          \
-    if (rows == 4) cudaLaunchKernelEx(&l.cfg, kv4_norm_rope_kernel<LPR, 4>, a); \
-    else cudaLaunchKernelEx(&l.cfg, kv4_norm_rope_kernel<LPR, 1>, a);
+#define VX_ROPE(LPR, F32)                                                                           \
+    if (rows != 1) cudaLaunchKernelEx(&l.cfg, kv4_norm_rope_kernel<LPR, rope_rows(F32), F32>, a);   \
+    else cudaLaunchKernelEx(&l.cfg, kv4_norm_rope_kernel<LPR, 1, F32>, a);
     if (a.head_dim == 128) {
-        VX_ROPE(16)
+        if (a.in_f32) { VX_ROPE(16, true) } else { VX_ROPE(16, false) }
     } else {
-        VX_ROPE(8)
+        if (a.in_f32) { VX_ROPE(8, true) } else { VX_ROPE(8, false) }
     }
 #undef VX_ROPE
     return launch_status();
 }
 
 // ---- exact read of rows ---------------------------------------------------------------------------
-// One thread per eight values of a row (four code bytes): value = (code * scale) / divisor; the
-// product is exact (six significant bits), the quotient is rounded once to f32, then to the output.
+// A warp takes the K and the V rows of 16 * 8 / D heads of a token, a lane eight values of a row (four
+// code bytes): value = (code * scale) / divisor; the product is exact (six significant bits), the quotient
+// rounded once to f32, then to the output's type.
+template <int LPR>
 __global__ void __launch_bounds__(256)
 kv4_rows_kernel(Kv4Geom c, const int32_t* __restrict__ slots, int tokens, void* k_out, void* v_out, int out_f32) {
-    const int D = c.head_dim, per_row = D / 8;
+    constexpr int D = LPR * 8, HEADS = 16 / LPR;   // heads per warp
     if (threadIdx.x == 0) grid_launch_dependents();
     grid_dependency_wait();
-    const long long rows = (long long)tokens * c.kv_heads;
-    const long long total = rows * per_row * 2, cap = c.pages * c.page_size;
-    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const bool is_v = i >= total / 2;
-        const long long e = is_v ? i - total / 2 : i;
-        void* dst = is_v ? v_out : k_out;
-        if (!dst) continue;
-        const long long row = e / per_row;
-        const int w = (int)(e - row * per_row);
-        const long long tok = row / c.kv_heads;
-        const int h = (int)(row - tok * c.kv_heads);
+    const int lane = threadIdx.x & 31, w = lane % LPR, is_v = (lane / LPR) & 1, sub = lane / (2 * LPR);
+    const unsigned chunks = (c.kv_heads + HEADS - 1) / HEADS;
+    const unsigned total = (unsigned)tokens * chunks, stride = gridDim.x * 8;
+    const long long cap = c.pages * c.page_size;
+    void* dst = is_v ? v_out : k_out;
+    const float div = is_v ? c.v_div : c.k_div, r = __fdiv_rn(1.0f, div);
+    for (unsigned task = blockIdx.x * 8 + (threadIdx.x >> 5); task < total; task += stride) {
+        const unsigned tok = task / chunks;
+        const int h = (int)(task - tok * chunks) * HEADS + sub;
         const int slot = slots[tok];
-        if (slot < 0 || slot >= cap) continue;   // a row that is not in the cache: left as it was
-        int tau;
-        const uint8_t* blk = kv4_block_of(c, slot, h, tau);
-        const uint32_t codes = *reinterpret_cast<const uint32_t*>(blk + (is_v ? kv4_v_code(D, tau, w * 4) : kv4_k_code(D, tau, w * 4)));
-        const float s = e4m3_to_f32(blk[is_v ? kv4_v_scale(D, tau, w >> 1) : kv4_k_scale(D, tau, w >> 1)] & 0x7fu);
-        const float div = is_v ? c.v_div : c.k_div;
-        float x[8];
+        if (slot >= 0 && slot < cap && h < c.kv_heads && dst) {   // (a row that is not in the cache: left as it was)
+            int tau;
+            const uint8_t* blk = kv4_block_of(c, slot, h, tau);
+            const uint32_t codes = *reinterpret_cast<const uint32_t*>(blk + (is_v ? kv4_v_code(D, tau, w * 4) : kv4_k_code(D, tau, w * 4)));
+            const float s = e4m3_to_f32(blk[is_v ? kv4_v_scale(D, tau, w >> 1) : kv4_k_scale(D, tau, w >> 1)] & 0x7fu);
+            float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = __fdiv_rn(e2m1_to_f32(codes >> (4 * j) & 15u) * s, div);
-        store_row8(dst, row * D + w * 8, out_f32, x);
+            for (int j = 0; j < 8; j++) x[j] = quotient(e2m1_to_f32(codes >> (4 * j) & 15u) * s, div, r);
+            store_row8(dst, ((long long)tok * c.kv_heads + h) * D + w * 8, out_f32, x);
+        }
     }
 }
 
 int kv4_rows(const Kv4Geom& c, const int32_t* slots, int tokens, void* k_out, void* v_out, int out_f32) {
-    const long long total = (long long)tokens * c.kv_heads * (c.head_dim / 8) * 2;
-    long long blocks = (total + 255) / 256;
-    if (blocks > 16LL * kv4_sms()) blocks = 16LL * kv4_sms();
+    const int heads = c.head_dim == 128 ? 1 : 2;
+    const long long tasks = (long long)tokens * ((c.kv_heads + heads - 1) / heads);
+    if (tasks > 0x7fffffffLL) return VELOX_ERR_UNSUPPORTED;
+    long long blocks = (tasks + 7) / 8;
+    if (blocks > 8LL * kv4_sms()) blocks = 8LL * kv4_sms();
     EarlyLaunch l((unsigned)blocks, 256);
-    cudaLaunchKernelEx(&l.cfg, kv4_rows_kernel, c, slots, tokens, k_out, v_out, out_f32);
+    if (c.head_dim == 128)
+        cudaLaunchKernelEx(&l.cfg, kv4_rows_kernel<16>, c, slots, tokens, k_out, v_out, out_f32);
+    else
+        cudaLaunchKernelEx(&l.cfg, kv4_rows_kernel<8>, c, slots, tokens, k_out, v_out, out_f32);
     return launch_status();
 }
 
