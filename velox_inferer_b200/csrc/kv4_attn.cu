@@ -12,10 +12,12 @@
 // largest). P is rounded to f16 (2^-11; probabilities are scaled by 2^8 so that small ones stay
 // normal), everything else is f32.
 //
-// Bytes reach the warps as MMA operands straight from global memory (the cache's block layout, kv4.cuh):
-// no shared memory, no barrier in the loop. The blocks of a step are requested as soon as the
-// registers that hold the step before are free, K during the softmax and V product, V during the
-// next K product.
+// Every warp streams its own blocks through a ring of its own in shared memory (cp.async, three steps of two
+// blocks: up to 147 KB per SM on their way), so there is no barrier in the loop. The block layout (kv4.cuh) makes
+// a lane's MMA operands one conflict-free access per plane. (Operands loaded straight into registers kept
+// half as much in flight: 126 us against XXX us for 64 requests of 4k to 8k tokens, 64 / 8 heads of 128.)
+// A block or page that is not there is read from the start of the cache instead (any byte is a finite
+// number) and its scores are masked.
 //
 // Work is cut by length, on the device (the lengths live there): all (request, kv head, row tile)
 // items are laid end to end in units of one tile of tokens, every block takes an equal run. A
@@ -39,6 +41,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+    const __nv_bfloat162 v = __float22bfloat162_rn(make_float2(lo, hi));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 template <int D, int NT, int WARPS>
 struct DecodeCfg {
     static constexpr int ROWS = 8 * NT;            // query rows of an item
@@ -46,10 +53,63 @@ struct DecodeCfg {
     static constexpr int TILE = WARPS * STEP;      // tokens per unit of work
     static constexpr int THREADS = WARPS * 32;
     static constexpr int STRIDE = D + 4;           // padded f32 row in shared memory
-    static constexpr int SMEM = WARPS * ROWS * STRIDE * 4 + 2 * WARPS * ROWS * 4;
+    static constexpr int BLOCK = 18 * D, STAGE = 2 * BLOCK, STAGES = 3;
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int JOIN = WARPS * ROWS * STRIDE * 4 + 2 * WARPS * ROWS * 4;   // over the ring
+    static constexpr int SMEM = RING > JOIN ? RING : JOIN;
     // a parked part: max, sum per row, then O
     static constexpr int PART = ROWS * (D + 2);
 };
+
+__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// The two blocks of a step into a stage, by the whole warp: 2 * 18 D bytes.
+template <int D>
+__device__ __forceinline__ void copy_step(uint32_t dst, const uint8_t* p0, const uint8_t* p1, int lane) {
+    constexpr int CHUNKS = 18 * D / 16, ALL = 2 * CHUNKS;   // 144 or 72 per block
+#pragma unroll
+    for (int i = 0; i < (ALL + 31) / 32; i++) {
+        const int c = lane + 32 * i;
+        const uint8_t* src = 32 * i + 31 < CHUNKS || (32 * i < CHUNKS && c < CHUNKS) ? p0 + c * 16 : p1 + (c - CHUNKS) * 16;
+        if (32 * i + 31 < ALL || c < ALL) copy16(dst + c * 16, src);
+    }
+}
+// A lane's operands of a block in shared memory.
+template <int D>
+__device__ __forceinline__ void lds_plane(uint32_t (&c)[2][D / 32], uint32_t p, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (D == 128) {
+            uint32_t v[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p + 512 * h + lane * 16));
+            c[h][0] = v[0]; c[h][1] = v[1]; c[h][D / 32 - 2] = v[2]; c[h][D / 32 - 1] = v[3];
+        } else {
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[h][0]), "=r"(c[h][1]) : "r"(p + 256 * h + lane * 8));
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ void lds_k(KRegs<D>& r, uint32_t blk, int lane) {
+    lds_plane<D>(r.c, blk, lane);
+    if (D == 128) {
+        r.s = lds4(blk + 16 * D + lane * 4);
+    } else {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(blk + 16 * D + lane * 2));
+        r.s = v;
+    }
+}
+template <int D>
+__device__ __forceinline__ void lds_v(VRegs<D>& r, uint32_t blk, int lane) {
+    lds_plane<D>(r.c, blk + 8 * D, lane);
+    r.s = lds4(blk + 17 * D + (D == 128 ? lane : (lane >> 3) * 4 + (lane & 3)) * 4);
+}
 
 // S^T of one block of 16 tokens: c[n] rows g, g + 8 = tokens, columns 2t, 2t + 1 of row tile n.
 template <int D, int NT>
@@ -113,23 +173,25 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1)
 kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using C = DecodeCfg<D, NT, WARPS>;
     constexpr int ROWS = C::ROWS, TILE = C::TILE;
-    extern __shared__ float smem[];
+    extern __shared__ __align__(16) float smem[];
     float* s_o = smem;                                   // [WARPS][ROWS][STRIDE]
     float* s_m = smem + WARPS * ROWS * C::STRIDE;        // [WARPS][ROWS] max, then sum
     __shared__ long long s_red[WARPS], s_found[2];
     __shared__ int s_last;
+    __shared__ float s_sum[ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = __ffs(a.cache.page_size) - 5;   // (blocks per page: a power of two)
     if (tid == 0) grid_launch_dependents();
     grid_dependency_wait();
 
-    const Run run = find_run<ROWS, TILE, C::THREADS>(a, G, s_red, s_found);
+    const Run run = find_run<ROWS, TILE, C::THREADS, 4>(a, G, s_red, s_found);
     if ((int)blockIdx.x >= run.blocks) return;
-    const int cta = blockIdx.x;
     const float soft = score_factor(a);
     uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws);
     float* parts = reinterpret_cast<float*>(a.ws + a.decode_parts);
 
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (tid >> 5) * (C::STAGES * C::STAGE);
+    int done = 0;
     Items<ROWS, TILE> it(a, G, run);
     for (; it.more(); it.next(a, G)) {
         const Request& r = it.r;
@@ -176,7 +238,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 qf[n][j][0] = pack_f16(x[4 * j] * down, x[4 * j + 1] * down);
                 qf[n][j][1] = pack_f16(x[4 * j + 2] * down, x[4 * j + 3] * down);
             }
-            const float up = soft * pow2(e);
+            const float up = fmaxf(soft * pow2(e), 1e-37f);   // (a factor of 0 would turn masked scores into NaN)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int col = n * 8 + 2 * t + c;
@@ -199,54 +261,68 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int i = 0; i < D / 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
 
-        // Page ids of this warp's next sixteen steps: lane i holds the id of block i & 1 of step i / 2.
+        // Page ids of this warp's next sixteen steps, and of the sixteen after them: lane i holds the id of block
+        // i & 1 of step i / 2.
         const int32_t* trow = a.table + (long long)b * a.cols;
         const int blk_hi = (range.hi + 15) >> 4;
+        const int kb0 = tile0 * (TILE / 16) + warp * 2;   // first block of step 0
         auto page_of = [&](int k) {
-            const int kb = (tile0 + k + (lane >> 1)) * (TILE / 16) + warp * 2 + (lane & 1);
-            return kb < blk_hi ? trow[kb >> page_shift] : -1;
+            const int kb = kb0 + (k + (lane >> 1)) * (TILE / 16) + (lane & 1);
+            return kb < blk_hi && k + (lane >> 1) < k1 ? trow[kb >> page_shift] : -1;
         };
-        auto block_at = [&](int id, int k, int which) -> const uint8_t* {
-            if (id < 0 || id >= a.cache.pages) return nullptr;
-            const int kb = (tile0 + k) * (TILE / 16) + warp * 2 + which;
-            return a.cache.blocks + ((((long long)id * hkv + h) << page_shift) + (kb & ((1 << page_shift) - 1))) * (18 * D);
-        };
-        int ids = page_of(k0), ids_at = k0;
-        const uint8_t* blk[2];
-        KRegs<D> kr[2];
-        VRegs<D> vr[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            blk[i] = block_at(__shfl_sync(0xffffffffu, ids, i), k0, i);
-            load_k<D>(kr[i], blk[i], lane);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++) load_v<D>(vr[i], blk[i], lane);
-
-        for (int k = k0; k < k1; k++) {
-            float c[2][NT][4];
-            const bool have0 = blk[0] != nullptr, have1 = blk[1] != nullptr;
-#pragma unroll
-            for (int i = 0; i < 2; i++) scores<D, NT>(kr[i], qf, c[i]);
-            if (k + 1 < k1) {   // K of the next step
-                if (k + 1 - ids_at == 16) {
-                    ids_at = k + 1;
-                    ids = page_of(ids_at);
+        int ids = page_of(k0), ids_next = page_of(k0 + 16);
+        const uint8_t* head = a.cache.blocks + ((long long)h << page_shift) * C::BLOCK;
+        const long long page_bytes = ((long long)hkv << page_shift) * C::BLOCK;
+        uint32_t have = 0;        // two bits per step on its way, the oldest lowest
+        int issued = k0, slot_in = 0;
+        __syncthreads();          // (the ring is the join's memory of the item before)
+        auto issue = [&]() {
+            if (issued < k1) {
+                const int at = (issued - k0) & 15;
+                if (at == 0 && issued != k0) {
+                    ids = ids_next;
+                    ids_next = page_of(issued + 16);
                 }
+                const uint8_t* p[2];
+                uint32_t bits = 0;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    blk[i] = block_at(__shfl_sync(0xffffffffu, ids, (k + 1 - ids_at) * 2 + i), k + 1, i);
-                    load_k<D>(kr[i], blk[i], lane);
+                    const int id = __shfl_sync(0xffffffffu, ids, at * 2 + i);
+                    const int kb = kb0 + issued * (TILE / 16) + i;
+                    const bool there = (uint32_t)id < (uint32_t)a.cache.pages;
+                    bits |= there ? 1u << i : 0u;
+                    p[i] = head + (there ? id : 0) * page_bytes + (kb & ((1 << page_shift) - 1)) * C::BLOCK;
                 }
+                have |= bits << (2 * (issued - done));
+                copy_step<D>(ring + slot_in * C::STAGE, p[0], p[1], lane);
+                slot_in = slot_in == C::STAGES - 1 ? 0 : slot_in + 1;
+            }
+            issued++;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        done = k0;
+#pragma unroll
+        for (int i = 0; i < C::STAGES - 1; i++) issue();
+
+        int slot = 0;
+        for (int k = k0; k < k1; k++) {
+            issue();
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
+            __syncwarp();
+            const uint32_t stage = ring + slot * C::STAGE;
+            slot = slot == C::STAGES - 1 ? 0 : slot + 1;
+            const uint32_t there = have & 3u;
+            have >>= 2;
+            done = k + 1;
+            float c[2][NT][4];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                KRegs<D> kr;
+                lds_k<D>(kr, stage + i * C::BLOCK, lane);
+                scores<D, NT>(kr, qf, c[i]);
             }
             const int tok = (tile0 + k) * TILE + warp * 32;
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) c[i][n][x] *= ksc[n][x & 1];
-            if (tok < all_lo || tok + 32 > all_hi || !have0 || !have1) {
+            if (tok < all_lo || tok + 32 > all_hi || there != 3u) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -254,8 +330,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
                         for (int x = 0; x < 4; x++) {
                             const int j = tok + i * 16 + g + (x >> 1) * 8;
-                            if (j < lim_lo[n][x & 1] || j >= lim_hi[n][x & 1] || !(i == 0 ? have0 : have1))
-                                c[i][n][x] = -INFINITY;
+                            if (j < lim_lo[n][x & 1] || j >= lim_hi[n][x & 1] || !(there >> i & 1u)) c[i][n][x] = -INFINITY;
                         }
             }
             // running maximum of each row (column of S^T), over the lanes that share the column
@@ -266,9 +341,9 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    float v = fmaxf(fmaxf(c[0][n][y], c[0][n][y + 2]), fmaxf(c[1][n][y], c[1][n][y + 2]));
-                    grew = grew || v > m[n][y];
-                    mx[n][y] = v;
+                    const float v = fmaxf(fmaxf(c[0][n][y], c[0][n][y + 2]), fmaxf(c[1][n][y], c[1][n][y + 2]));
+                    mx[n][y] = v * ksc[n][y];
+                    grew = grew || mx[n][y] > m[n][y];
                 }
             if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -290,80 +365,94 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     }
             }
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int n = 0; n < NT; n++) {
+                const float off[2] = {8.0f - m[n][0], 8.0f - m[n][1]};
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
+                for (int i = 0; i < 2; i++) {
                     float p[4];
 #pragma unroll
-                    for (int x = 0; x < 4; x++) p[x] = exp2_approx(c[i][n][x] - m[n][x & 1] + 8.0f);
+                    for (int x = 0; x < 4; x++) p[x] = exp2_approx(fmaf(c[i][n][x], ksc[n][x & 1], off[x & 1]));
                     l[n][0] += p[0] + p[2];
                     l[n][1] += p[1] + p[3];
                     pf[i][n][0] = transpose8x8(pack_f16(p[0], p[1]));
                     pf[i][n][1] = transpose8x8(pack_f16(p[2], p[3]));
                 }
-#pragma unroll
-            for (int i = 0; i < 2; i++) accumulate<D, NT>(vr[i], pf[i], o);
-            if (k + 1 < k1) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) load_v<D>(vr[i], blk[i], lane);
             }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                VRegs<D> vr;
+                lds_v<D>(vr, stage + i * C::BLOCK, lane);
+                accumulate<D, NT>(vr, pf[i], o);
+            }
+            __syncwarp();   // before the stage is written again
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
 
         // ---- join the warps ----
-        __syncthreads();   // (shared memory of the item before)
+        // Rows are kept in the order [i][g][2]: dimension g * D/8 + 2i + e at i * 16 + 2g + e; a thread joins four
+        // neighbours of it.
+        __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                float s = l[n][y];
-                s += __shfl_xor_sync(0xffffffffu, s, 4);
-                s += __shfl_xor_sync(0xffffffffu, s, 8);
-                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                float sum = l[n][y];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int row = n * 8 + 2 * t + y;
                 if (g == 0) {
                     s_m[warp * ROWS + row] = m[n][y];
-                    s_m[(WARPS + warp) * ROWS + row] = s;
+                    s_m[(WARPS + warp) * ROWS + row] = sum;
                 }
-            }
-        // rows in the order [i][g][2]: dimension g * D/8 + 2i + e at i * 16 + 2g + e
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                for (int y = 0; y < 2; y++)
-                    *reinterpret_cast<float2*>(s_o + (warp * ROWS + n * 8 + 2 * t + y) * C::STRIDE + i * 16 + 2 * g) =
+                for (int i = 0; i < D / 16; i++)
+                    *reinterpret_cast<float2*>(s_o + (warp * ROWS + row) * C::STRIDE + i * 16 + 2 * g) =
                         make_float2(o[n][i][y], o[n][i][y + 2]);
-        __syncthreads();
+            }
         const bool whole = it.whole();
-        const int c_first = it.first_block(), c_last = it.last_block();
-        float* part = parts + ((long long)cta * 2 + (cta == c_first ? 1 : 0)) * C::PART;
-        for (int i = tid; i < ROWS * D; i += C::THREADS) {
-            const int row = i / D, d = i % D;
-            const int at = (d % (D / 8)) / 2 * 16 + d / (D / 8) * 2 + (d & 1);
-            float mm = NEG_BIG;
+        const int c_first = whole ? 0 : it.first_block(), c_last = whole ? 0 : it.last_block();
+        float* part = parts + ((long long)blockIdx.x * 2 + ((int)blockIdx.x == c_first ? 1 : 0)) * C::PART;
+        __syncthreads();
+        if (tid < ROWS) {   // the warps' factors, and the row's maximum and sum
+            float mm = NEG_BIG, ll = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, s_m[w * ROWS + row]);
-            float acc = 0.0f, ll = 0.0f;
+            for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, s_m[w * ROWS + tid]);
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
-                const float f = exp2_approx(s_m[w * ROWS + row] - mm);
-                acc += f * s_o[(w * ROWS + row) * C::STRIDE + at];
-                ll += f * s_m[(WARPS + w) * ROWS + row];
+                const float f = exp2_approx(s_m[w * ROWS + tid] - mm);
+                ll += f * s_m[(WARPS + w) * ROWS + tid];
+                s_m[w * ROWS + tid] = f;
             }
-            if (whole) {
-                if (row < rows) {
-                    const int rr = rt * ROWS + row;
-                    a.out[(long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d] =
-                        bf16_bits(finish(acc, ll, a.cache.v_div));
-                }
-            } else {
-                part[2 * ROWS + i] = acc;
-                if (d == 0) {
-                    part[row] = mm;
-                    part[ROWS + row] = ll;
-                }
+            s_sum[tid] = finish(1.0f, ll, a.cache.v_div);
+            if (!whole) {
+                part[tid] = mm;
+                part[ROWS + tid] = ll;
             }
+        }
+        __syncthreads();
+        auto write = [&](int row, int at, const float4& v, float inv) {   // four results of a row that exists
+            const int rr = rt * ROWS + row, d = (at & 15) / 2 * (D / 8) + at / 16 * 2;
+            uint16_t* dst = a.out + (long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d;
+            *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(v.x * inv, v.y * inv);
+            *reinterpret_cast<uint32_t*>(dst + D / 8) = pack_bf16x2(v.z * inv, v.w * inv);
+        };
+        for (int i = tid; i < ROWS * D / 4; i += C::THREADS) {
+            const int row = i / (D / 4), at = i % (D / 4) * 4;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float f = s_m[w * ROWS + row];
+                const float4 v = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * C::STRIDE + at);
+                acc.x += f * v.x;
+                acc.y += f * v.y;
+                acc.z += f * v.z;
+                acc.w += f * v.w;
+            }
+            if (!whole)
+                *reinterpret_cast<float4*>(part + 2 * ROWS + row * D + at) = acc;
+            else if (row < rows)
+                write(row, at, acc, s_sum[row]);
         }
         if (!whole) {
             __threadfence();
@@ -373,21 +462,41 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             if (s_last) {   // the item's last block: join the parts in token order
                 __threadfence();
                 if (tid == 0) tickets[c_first] = 0;
-                for (int i = tid; i < rows * D; i += C::THREADS) {
-                    const int row = i / D, d = i % D;
-                    float mm = NEG_BIG, acc = 0.0f, ll = 0.0f;
-                    for (int c = c_first; c <= c_last; c++) {
-                        const float* q = parts + ((long long)c * 2 + (c == c_first ? 1 : 0)) * C::PART;
-                        const float pm = __ldcg(q + row), pl = __ldcg(q + ROWS + row), po = __ldcg(q + 2 * ROWS + i);
-                        const float v = fmaxf(mm, pm);
-                        const float f0 = exp2_approx(mm - v), f1 = exp2_approx(pm - v);
-                        acc = acc * f0 + po * f1;
-                        ll = ll * f0 + pl * f1;
-                        mm = v;
+                const int count = c_last - c_first + 1;
+                auto part_of = [&](int c) { return parts + ((long long)(c_first + c) * 2 + (c == 0 ? 1 : 0)) * C::PART; };
+                float* s_f = smem;                      // [count][ROWS]: maxima, then factors
+                float* s_l = smem + count * ROWS;       // sums
+                for (int i = tid; i < count * ROWS; i += C::THREADS) {
+                    s_f[i] = __ldcg(part_of(i / ROWS) + i % ROWS);
+                    s_l[i] = __ldcg(part_of(i / ROWS) + ROWS + i % ROWS);
+                }
+                __syncthreads();
+                for (int row = warp; row < ROWS; row += WARPS) {
+                    float mm = NEG_BIG, ll = 0.0f;
+                    for (int c = lane; c < count; c += 32) mm = fmaxf(mm, s_f[c * ROWS + row]);
+                    mm = warp_max(mm);
+                    for (int c = lane; c < count; c += 32) {
+                        const float f = exp2_approx(s_f[c * ROWS + row] - mm);
+                        ll += f * s_l[c * ROWS + row];
+                        s_f[c * ROWS + row] = f;
                     }
-                    const int rr = rt * ROWS + row;
-                    a.out[(long long)(r.row0 + rr / G) * a.out_stride + (long long)(h * G + rr % G) * D + d] =
-                        bf16_bits(finish(acc, ll, a.cache.v_div));
+                    ll = warp_sum(ll);
+                    if (lane == 0) s_sum[row] = finish(1.0f, ll, a.cache.v_div);
+                }
+                __syncthreads();
+                for (int i = tid; i < rows * D / 4; i += C::THREADS) {
+                    const int row = i / (D / 4), at = i % (D / 4) * 4;
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                    for (int c = 0; c < count; c++) {
+                        const float f = s_f[c * ROWS + row];
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(c) + 2 * ROWS + row * D + at));
+                        acc.x += f * v.x;
+                        acc.y += f * v.y;
+                        acc.z += f * v.z;
+                        acc.w += f * v.w;
+                    }
+                    write(row, at, acc, s_sum[row]);
                 }
             }
         }

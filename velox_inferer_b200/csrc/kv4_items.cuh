@@ -80,7 +80,16 @@ struct Run {
     int blocks;    // blocks that have a run
     int request;
 };
-template <int ROWS, int TILE, int THREADS>
+// total * i / n; 64-bit divisions are slow, and most totals are small
+__device__ __forceinline__ long long share(long long total, int i, int n) {
+    return total < 1 << 20 ? (long long)((uint32_t)total * (uint32_t)i / (uint32_t)n) : total * i / n;   // (n < 2^12)
+}
+// First block whose run ends after unit u.
+__device__ __forceinline__ int block_of(long long u, long long total, int n) {
+    return (total < 1 << 20 ? (int)(((uint32_t)(u + 1) * (uint32_t)n + (uint32_t)total - 1) / (uint32_t)total)
+                            : (int)(((u + 1) * n + total - 1) / total)) - 1;
+}
+template <int ROWS, int TILE, int THREADS, int MIN_RUN>
 __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* red, long long* found) {
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hkv = a.cache.kv_heads;
@@ -98,12 +107,13 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     run.total = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; i++) run.total += red[i];
-    run.blocks = (int)min((long long)gridDim.x, run.total);
+    // Short runs cost more to join than they save: at least MIN_RUN units per block.
+    run.blocks = (int)min((long long)gridDim.x, (run.total + MIN_RUN - 1) / MIN_RUN);
     run.request = 0;
     run.request_first = run.begin = run.end = 0;
     if ((int)blockIdx.x >= run.blocks) return run;
-    run.begin = run.total * blockIdx.x / run.blocks;
-    run.end = run.total * (blockIdx.x + 1) / run.blocks;
+    run.begin = share(run.total, blockIdx.x, run.blocks);
+    run.end = share(run.total, blockIdx.x + 1, run.blocks);
     long long before = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
         const int b = base + tid;
@@ -208,8 +218,8 @@ struct Items {
     }
     __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nt; }
     // First and last block that hold a part of this item.
-    __device__ __forceinline__ int first_block() const { return (int)(((item_first + 1) * blocks + total - 1) / total) - 1; }
-    __device__ __forceinline__ int last_block() const { return (int)(((item_first + nt) * blocks + total - 1) / total) - 1; }
+    __device__ __forceinline__ int first_block() const { return block_of(item_first, total, blocks); }
+    __device__ __forceinline__ int last_block() const { return block_of(item_first + nt - 1, total, blocks); }
 };
 
 // ---- reading the cache -------------------------------------------------------------------------

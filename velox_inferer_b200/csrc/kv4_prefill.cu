@@ -184,7 +184,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     }
     tc_fence_before();
     grid_dependency_wait();
-    const Run run = find_run<PF_ROWS, PF_TILE, PF_THREADS>(a, G, s_red, s_found);
+    const Run run = find_run<PF_ROWS, PF_TILE, PF_THREADS, 4>(a, G, s_red, s_found);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
