@@ -324,6 +324,20 @@ def test_attention(case):
     check(cache, table, cu, lens, q, again, 0.75, D ** -0.5, causal, window)
 
 
+@pytest.mark.parametrize("requests", [33, 64, 257, 300, 513, 700])
+@pytest.mark.parametrize("new", [1, 30])
+def test_attention_many_requests(requests, new):
+    """More requests than a warp, a block of the decode kernel (256) and one of the prefill kernel (512) count at once."""
+    b = backend()
+    rng = np.random.default_rng(requests)
+    fresh = rng.integers(0, 2, requests) if new == 1 else np.where(rng.random(requests) < 0.1, rng.integers(17, new + 1, requests), 1)
+    lens = fresh + rng.integers(0, 40, requests)
+    cache, table, cu, q, T = scene(list(lens), list(fresh), 2, 1, 64, 16, requests, 2)
+    out = torch.full((T, 2, 64), 0.75, dtype=torch.bfloat16, device=DEV)
+    b.kv4_attention(q, out, cache, i32(table), i32(cu), i32(lens), b.kv4_workspace(2, 1, 64), max_new=int(fresh.max()))
+    check(cache, table, cu, lens, q, out, 0.75, 0.125, True, 0)
+
+
 @pytest.mark.parametrize("qscale,scale", [(1e-3, 1.0), (300.0, 0.02), (1e20, 1e-21), (0.0, 1.0)])
 def test_attention_query_ranges(qscale, scale):
     b = backend()

@@ -58,9 +58,10 @@ __device__ __forceinline__ long long warp_units(const Kv4AttnArgs& a, int G, int
 }
 // The same for a request per lane: a lane counts a single row tile itself, the warp together counts the others'.
 template <int ROWS, int TILE>
-__device__ __forceinline__ long long lane_units(const Kv4AttnArgs& a, int G, int b) {
+__device__ __forceinline__ long long lane_units(const Kv4AttnArgs& a, int G, int b, int& row_tiles) {
     Request r{};
     if (b < a.requests) r = request_of<ROWS>(a, G, b);
+    row_tiles = r.row_tiles;
     long long units = r.row_tiles == 1 ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0;
     uint32_t many = __ballot_sync(0xffffffffu, r.row_tiles > 1);
     while (many) {
@@ -95,10 +96,12 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hkv = a.cache.kv_heads;
     Run run;
     const bool once = a.requests <= THREADS;
+    constexpr int ITEMS = 40;   // items are counted above the units
+    int row_tiles;
     long long first = 0, mine = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
-        first = lane_units<ROWS, TILE>(a, G, base + tid) * hkv;
-        mine += first;
+        first = lane_units<ROWS, TILE>(a, G, base + tid, row_tiles) * hkv;
+        mine += first + ((long long)row_tiles * hkv << ITEMS);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -107,8 +110,10 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     run.total = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; i++) run.total += red[i];
-    // Short runs cost more to join than they save: at least MIN_RUN units per block.
-    run.blocks = (int)min((long long)gridDim.x, (run.total + MIN_RUN - 1) / MIN_RUN);
+    const long long items = run.total >> ITEMS;
+    run.total &= (1LL << ITEMS) - 1;
+    // Short runs of one item cost more to join than they save: MIN_RUN units per block, or an item each.
+    run.blocks = (int)min((long long)gridDim.x, max(items, (run.total + MIN_RUN - 1) / MIN_RUN));
     run.request = 0;
     run.request_first = run.begin = run.end = 0;
     if ((int)blockIdx.x >= run.blocks) return run;
@@ -117,7 +122,7 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     long long before = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
         const int b = base + tid;
-        const long long v = once ? first : lane_units<ROWS, TILE>(a, G, b) * hkv;
+        const long long v = once ? first : lane_units<ROWS, TILE>(a, G, b, row_tiles) * hkv;
         long long x = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -132,8 +137,9 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
         long long pre = before, sum = 0;
 #pragma unroll
         for (int i = 0; i < WARPS; i++) {
-            pre += i < warp ? red[i] : 0;
-            sum += red[i];
+            const long long units = red[i] & ((1LL << ITEMS) - 1);   // (the first pass's words count items too)
+            pre += i < warp ? units : 0;
+            sum += units;
         }
         const long long lo = pre + x - v;
         if (run.begin >= lo && run.begin < lo + v) {
