@@ -41,27 +41,23 @@ def _view_struct(w: WeightView) -> _lib.View:
                      w.rows, w.act.divisor)
 
 
-def _rows3(t: torch.Tensor, device, what: str, heads: int, head_dim: int, dtypes, tokens: int):
+def _rows3(t: torch.Tensor, index: int, what: str, heads: int, head_dim: int, dtype, tokens: int):
     """(address, elements between tokens) of a [tokens, heads, head_dim] operand whose heads are contiguous."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise ShapeError(f"{what}: expected a tensor on {device}")
-    if t.dtype not in dtypes:
-        raise ShapeError(f"{what}: expected {dtypes}, got {t.dtype}")
-    if t.shape != (tokens, heads, head_dim):
-        raise ShapeError(f"{what}: expected [{tokens}, {heads}, {head_dim}], got {tuple(t.shape)}")
-    s0, s1, s2 = t.stride()
-    if (s2 != 1 or (heads > 1 and s1 != head_dim)) and t.numel() > 0:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.shape == (tokens, heads, head_dim):
+        s0, s1, s2 = t.stride()
+        if (s2 == 1 and (s1 == head_dim or heads <= 1)) or tokens * heads == 0:
+            return t.data_ptr(), (s0 if tokens > 1 else heads * head_dim)
         raise ShapeError(f"{what}: the heads of a token have to be contiguous, strides {t.stride()}")
-    return t.data_ptr(), (s0 if tokens > 1 else heads * head_dim)
+    raise ShapeError(f"{what}: expected {dtype} [{tokens}, {heads}, {head_dim}] on cuda:{index}, got "
+                     f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t)}")
 
 
-def _ints(t: torch.Tensor, device, what: str, shape) -> int:
+def _ints(t: torch.Tensor, index: int, what: str, shape) -> int:
     """Address of a contiguous int32 tensor of this shape."""
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32 or not t.is_contiguous():
-        raise ShapeError(f"{what}: expected a contiguous int32 tensor on {device}")
-    if t.shape != shape:
-        raise ShapeError(f"{what}: expected {tuple(shape)}, got {tuple(t.shape)}")
-    return t.data_ptr()
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    raise ShapeError(f"{what}: expected contiguous int32 {tuple(shape)} on cuda:{index}, got "
+                     f"{(t.dtype, tuple(t.shape), t.device) if isinstance(t, torch.Tensor) else type(t)}")
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -437,37 +433,37 @@ class Sm100Backend:
         """Page table rows, slots and positions of one step from the requests' lengths. ``table`` [requests, cols] is
         extended in place with pages from ``free``, of which ``taken`` [1] are used up; their new number goes to
         ``taken_out`` (``taken`` itself if None)."""
-        dev, n = self.device, step.requests
+        dev, n = self.device.index, step.requests
         if page_size not in PAGE_SIZES:
             raise Unsupported(f"kv4_plan: page_size {page_size} (of {PAGE_SIZES})")
         if table.dim() != 2 or free.dim() != 1:
             raise ShapeError("kv4_plan: table is [requests, cols], free [pages]")
-        out = taken if taken_out is None else taken_out
+        cols, stock = table.shape[1], free.shape[0]
+        taken_ = _ints(taken, dev, "kv4_plan taken", (1,))
         args = (_ints(cached, dev, "kv4_plan cached", (n,)), _ints(new, dev, "kv4_plan new", (n,)), n,
-                _ints(table, dev, "kv4_plan table", (n, table.shape[1])), table.shape[1],
-                _ints(free, dev, "kv4_plan free", free.shape), free.shape[0], _ints(taken, dev, "kv4_plan taken", (1,)),
-                _ints(out, dev, "kv4_plan taken_out", (1,)), page_size, step.tokens, step.cu.data_ptr(),
-                step.kv_lens.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(), step.status.data_ptr(),
-                step.ticket.data_ptr())
+                _ints(table, dev, "kv4_plan table", (n, cols)), cols, _ints(free, dev, "kv4_plan free", (stock,)), stock, taken_,
+                taken_ if taken_out is None else _ints(taken_out, dev, "kv4_plan taken_out", (1,)), page_size, step.tokens,
+                *step.addresses)
         self._bind()
         status(self.lib.velox_sm100_kv4_plan(*args), "sm100 kv4_plan")
 
     def _rope_args(self, what, head_dim, q_weight, k_weight, rope, positions, tokens):
         """(q weight, k weight, table, its length, rotated dimensions, positions) as the C entry points take them."""
-        dev = self.device
+        dev, f32 = self.device.index, torch.float32
         for w in (q_weight, k_weight):
-            if w is not None and (w.device != dev or w.dtype != torch.float32 or w.shape != (head_dim,) or not w.is_contiguous()):
-                raise ShapeError(f"{what}: norm weights are contiguous f32 [{head_dim}] on {dev}")
+            if w is not None and not (w.dtype is f32 and w.get_device() == dev and w.shape == (head_dim,) and w.is_contiguous()):
+                raise ShapeError(f"{what}: norm weights are contiguous f32 [{head_dim}] on {self.device}")
         if rope is None:
-            length = rot = 0
+            table, length, rot = None, 0, 0
         else:
-            if rope.device != dev or rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous():
-                raise ShapeError(f"{what}: rope is a contiguous f32 [positions, rot] on {dev}")
-            length, rot = rope.shape
+            if not (rope.dtype is f32 and rope.get_device() == dev and rope.dim() == 2 and rope.is_contiguous()):
+                raise ShapeError(f"{what}: rope is a contiguous f32 [positions, rot] on {self.device}")
             if positions is None:
                 raise ShapeError(f"{what}: a rotation needs positions")
-        pos = None if positions is None else _ints(positions, dev, f"{what} positions", (tokens,))
-        return _ptr(q_weight), _ptr(k_weight), _ptr(rope), length, rot, pos
+            table = rope.data_ptr()
+            length, rot = rope.shape
+        return (None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), table, length,
+                rot, None if positions is None else _ints(positions, dev, what, (tokens,)))
 
     def qk_norm_rope(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor],
                      k_weight: Optional[torch.Tensor], rope: Optional[torch.Tensor], positions: Optional[torch.Tensor],
@@ -476,29 +472,30 @@ class Sm100Backend:
         """RMS norm and rotation of every head of q [tokens, heads, D] and k [tokens, kv_heads, D] in one pass, f32 or
         bf16 in and out. Either may be None, the weights (no norm) and ``rope`` (no rotation) too; outputs may be
         their inputs. Rows whose position is outside the table stay as they were."""
-        dev, what = self.device, "qk_norm_rope"
+        dev, what = self.device.index, "qk_norm_rope"
         x, y = (q, q_out) if q is not None else (k, k_out)
-        if x is None or y is None or x.dim() != 3:
+        if x is None or y is None or x.dim() != 3 or (k is not None and k.dim() != 3):
             raise ShapeError(f"{what}: q or k as [tokens, heads, head_dim], and an output for it")
         if (q is None) != (q_out is None) or (k is None) != (k_out is None):
             raise ShapeError(f"{what}: every input has an output")
         tokens, _, D = x.shape
+        dt, odt = x.dtype, y.dtype
+        if dt not in _FLOATS or odt not in _FLOATS:
+            raise ShapeError(f"{what}: f32 or bf16, got {dt} -> {odt}")
         qp = kp = qo = ko = None
         qs = ks = qos = kos = hq = hk = 0
         if q is not None:
             hq = q.shape[1]
-            qp, qs = _rows3(q, dev, f"{what} q", hq, D, (x.dtype,), tokens)
-            qo, qos = _rows3(q_out, dev, f"{what} q_out", hq, D, (y.dtype,), tokens)
+            qp, qs = _rows3(q, dev, "qk_norm_rope q", hq, D, dt, tokens)
+            qo, qos = _rows3(q_out, dev, "qk_norm_rope q_out", hq, D, odt, tokens)
         if k is not None:
-            hk = k.shape[1] if k.dim() == 3 else -1
-            kp, ks = _rows3(k, dev, f"{what} k", hk, D, (x.dtype,), tokens)
-            ko, kos = _rows3(k_out, dev, f"{what} k_out", hk, D, (y.dtype,), tokens)
-        if x.dtype not in _FLOATS or y.dtype not in _FLOATS:
-            raise ShapeError(f"{what}: f32 or bf16, got {x.dtype} -> {y.dtype}")
+            hk = k.shape[1]
+            kp, ks = _rows3(k, dev, "qk_norm_rope k", hk, D, dt, tokens)
+            ko, kos = _rows3(k_out, dev, "qk_norm_rope k_out", hk, D, odt, tokens)
         qw, kw, rp, length, rot, pos = self._rope_args(what, D, q_weight, k_weight, rope, positions, tokens)
         self._bind()
-        status(self.lib.velox_sm100_qk_norm_rope(qp, qs, kp, ks, x.dtype == torch.float32, qw, kw, rp, length, rot, interleaved,
-                                                 pos, qo, qos, ko, kos, y.dtype == torch.float32, tokens, hq, hk, D, eps,
+        status(self.lib.velox_sm100_qk_norm_rope(qp, qs, kp, ks, dt is torch.float32, qw, kw, rp, length, rot, interleaved,
+                                                 pos, qo, qos, ko, kos, odt is torch.float32, tokens, hq, hk, D, eps,
                                                  offset), "sm100 qk_norm_rope")
 
     def qk_norm_rope_kv4(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
@@ -508,30 +505,32 @@ class Sm100Backend:
                          interleaved: bool = False) -> None:
         """The same pass with k and v quantised into the cache at ``slots`` [tokens] (-1: not written). No two rows of
         a call may share a slot."""
-        dev, what, D, hk = self.device, "qk_norm_rope_kv4", cache.head_dim, cache.kv_heads
-        if k.dim() != 3 or (q is None) != (q_out is None):
+        dev, what, D, hk = self.device.index, "qk_norm_rope_kv4", cache.head_dim, cache.kv_heads
+        if k.dim() != 3 or (q is None) != (q_out is None) or (q is not None and q.dim() != 3):
             raise ShapeError(f"{what}: k as [tokens, kv_heads, head_dim], and an output with q")
-        if cache.storage.device != dev:
+        if cache.device_index != dev:
             raise ShapeError(f"{what}: the cache is on {cache.storage.device}")
         tokens, dt = k.shape[0], k.dtype
         if dt not in _FLOATS:
             raise ShapeError(f"{what}: f32 or bf16, got {dt}")
-        kp, ks = _rows3(k, dev, f"{what} k", hk, D, (dt,), tokens)
-        vp, vs = _rows3(v, dev, f"{what} v", hk, D, (dt,), tokens)
+        kp, ks = _rows3(k, dev, "qk_norm_rope_kv4 k", hk, D, dt, tokens)
+        vp, vs = _rows3(v, dev, "qk_norm_rope_kv4 v", hk, D, dt, tokens)
         qp = qo = None
         qs = qos = hq = 0
         out_f32 = False
         if q is not None:
-            hq = q.shape[1] if q.dim() == 3 else -1
-            qp, qs = _rows3(q, dev, f"{what} q", hq, D, (dt,), tokens)
-            qo, qos = _rows3(q_out, dev, f"{what} q_out", hq, D, _FLOATS, tokens)
-            out_f32 = q_out.dtype == torch.float32
+            hq, odt = q.shape[1], q_out.dtype
+            if odt not in _FLOATS:
+                raise ShapeError(f"{what}: f32 or bf16, got {odt}")
+            qp, qs = _rows3(q, dev, "qk_norm_rope_kv4 q", hq, D, dt, tokens)
+            qo, qos = _rows3(q_out, dev, "qk_norm_rope_kv4 q_out", hq, D, odt, tokens)
+            out_f32 = odt is torch.float32
         qw, kw, rp, length, rot, pos = self._rope_args(what, D, q_weight, k_weight, rope, positions, tokens)
-        sl = _ints(slots, dev, f"{what} slots", (tokens,))
+        sl = _ints(slots, dev, "qk_norm_rope_kv4 slots", (tokens,))
         self._bind()
-        status(self.lib.velox_sm100_qk_norm_rope_kv4(qp, qs, kp, ks, vp, vs, dt == torch.float32, qw, kw, rp, length, rot,
-                                                     interleaved, pos, sl, C.byref(cache.struct), qo, qos, out_f32, tokens, hq,
-                                                     eps, offset), "sm100 qk_norm_rope_kv4")
+        status(self.lib.velox_sm100_qk_norm_rope_kv4(qp, qs, kp, ks, vp, vs, dt is torch.float32, qw, kw, rp, length, rot,
+                                                     interleaved, pos, sl, cache.ref, qo, qos, out_f32, tokens, hq, eps,
+                                                     offset), "sm100 qk_norm_rope_kv4")
 
     def kv4_store(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Kv4Cache) -> None:
         """k and v [tokens, kv_heads, D] quantised into the cache as they are."""
@@ -540,20 +539,20 @@ class Sm100Backend:
     def kv4_rows(self, cache: Kv4Cache, slots: torch.Tensor, k_out: Optional[torch.Tensor],
                  v_out: Optional[torch.Tensor]) -> None:
         """Exact decode of the cached rows at ``slots`` to [tokens, kv_heads, D], f32 or bf16 (either may be None)."""
-        dev, what = self.device, "kv4_rows"
+        dev, what = self.device.index, "kv4_rows"
         x = k_out if k_out is not None else v_out
-        if x is None or x.dtype not in _FLOATS or cache.storage.device != dev:
-            raise ShapeError(f"{what}: f32 or bf16 outputs and a cache on {dev}")
-        tokens = slots.shape[0] if slots.dim() == 1 else -1
+        if x is None or x.dtype not in _FLOATS or cache.device_index != dev or slots.dim() != 1:
+            raise ShapeError(f"{what}: f32 or bf16 outputs, slots [tokens] and a cache on {self.device}")
+        tokens, dt = slots.shape[0], x.dtype
         for t in (k_out, v_out):
             if t is not None:
-                _rows3(t, dev, what, cache.kv_heads, cache.head_dim, (x.dtype,), tokens)
+                _rows3(t, dev, what, cache.kv_heads, cache.head_dim, dt, tokens)
                 if not t.is_contiguous():
                     raise ShapeError(f"{what}: outputs are contiguous")
-        sl = _ints(slots, dev, f"{what} slots", (tokens,))
+        sl = _ints(slots, dev, "kv4_rows slots", (tokens,))
         self._bind()
-        status(self.lib.velox_sm100_kv4_rows(C.byref(cache.struct), sl, tokens, _ptr(k_out), _ptr(v_out),
-                                             x.dtype == torch.float32), "sm100 kv4_rows")
+        status(self.lib.velox_sm100_kv4_rows(cache.ref, sl, tokens, _ptr(k_out), _ptr(v_out), dt is torch.float32),
+               "sm100 kv4_rows")
 
     def kv4_workspace(self, heads: int, kv_heads: int, head_dim: int) -> torch.Tensor:
         """Workspace of ``kv4_attention``. Calls that may run at the same time (streams, captured graphs) need one each."""
@@ -570,19 +569,21 @@ class Sm100Backend:
         last of request b's kv_lens[b] tokens. ``scale``: D ** -0.5 if None. ``window``: a row sees that many tokens up to
         itself (0: all). ``max_new``: the largest number of new rows of a request, as far as the caller knows it
         (decode steps: 1); requests with more are left out. ``out`` is not ``q``."""
-        dev, what, D = self.device, "kv4_attention", cache.head_dim
-        if q.dim() != 3 or table.dim() != 2 or kv_lens.dim() != 1:
-            raise ShapeError(f"{what}: q [tokens, heads, head_dim], table [requests, cols], kv_lens [requests]")
+        dev, what, D, bf = self.device.index, "kv4_attention", cache.head_dim, torch.bfloat16
+        if q.dim() != 3 or table.dim() != 2:
+            raise ShapeError(f"{what}: q [tokens, heads, head_dim], table [requests, cols]")
         tokens, heads, _ = q.shape
         n, cols = table.shape
-        qp, qs = _rows3(q, dev, f"{what} q", heads, D, (torch.bfloat16,), tokens)
-        op, os_ = _rows3(out, dev, f"{what} out", heads, D, (torch.bfloat16,), tokens)
+        qp, qs = _rows3(q, dev, "kv4_attention q", heads, D, bf, tokens)
+        op, os_ = _rows3(out, dev, "kv4_attention out", heads, D, bf, tokens)
         if op == qp and tokens:
             raise ShapeError(f"{what}: out is q")
-        if cache.storage.device != dev or workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-            raise ShapeError(f"{what}: cache and workspace (uint8) on {dev}")
-        args = (qp, qs, op, os_, C.byref(cache.struct), _ints(table, dev, f"{what} table", (n, cols)), cols,
-                _ints(cu, dev, f"{what} cu", (n + 1,)), _ints(kv_lens, dev, f"{what} kv_lens", (n,)), n, tokens, heads,
+        if cache.device_index != dev or workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+            raise ShapeError(f"{what}: cache and workspace (uint8) on {self.device}")
+        if heads % cache.kv_heads != 0:
+            raise ShapeError(f"{what}: {heads} heads over {cache.kv_heads}")
+        args = (qp, qs, op, os_, cache.ref, _ints(table, dev, "kv4_attention table", (n, cols)), cols,
+                _ints(cu, dev, "kv4_attention cu", (n + 1,)), _ints(kv_lens, dev, "kv4_attention kv_lens", (n,)), n, tokens, heads,
                 D ** -0.5 if scale is None else scale, causal, window, tokens if max_new is None else max_new,
                 workspace.data_ptr(), workspace.numel())
         self._bind()

@@ -5,6 +5,7 @@ tables of its paged cache; format and layout are this library's own (include/vel
 as in the weights, 4.5 bits per value."""
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional
 
 import torch
@@ -23,7 +24,8 @@ class Kv4Cache:
     magnitude is a is stored with the scale e4m3(divisor * a / 6), so magnitudes from 6 * 2**-6 / divisor up to
     2688 / divisor keep the scale's full precision (16: from 0.006 to 168)."""
 
-    __slots__ = ("storage", "page_size", "head_dim", "kv_heads", "pages", "k_divisor", "v_divisor", "struct")
+    __slots__ = ("storage", "page_size", "head_dim", "kv_heads", "pages", "k_divisor", "v_divisor", "struct", "ref",
+                 "device_index")
 
     def __init__(self, storage: torch.Tensor, page_size: int, head_dim: int, k_divisor: float = 16.0,
                  v_divisor: float = 16.0):
@@ -43,6 +45,8 @@ class Kv4Cache:
         self.k_divisor, self.v_divisor = float(k_divisor), float(v_divisor)
         self.struct = _lib.Kv4CacheStruct(storage.data_ptr(), pages, page_size, kv_heads, head_dim, self.k_divisor,
                                           self.v_divisor, 0)
+        self.ref = C.byref(self.struct)
+        self.device_index = storage.get_device()
 
     @classmethod
     def alloc(cls, backend, pages: int, page_size: int, kv_heads: int, head_dim: int, k_divisor: float = 16.0,
@@ -60,7 +64,7 @@ class Kv4Step:
     """What ``Sm100Backend.kv4_plan`` writes for one step: ``cu`` [requests + 1], ``kv_lens`` [requests],
     ``positions`` and ``slots`` [tokens], ``status`` [1], all int32 on the device."""
 
-    __slots__ = ("cu", "kv_lens", "positions", "slots", "status", "ticket", "requests", "tokens")
+    __slots__ = ("cu", "kv_lens", "positions", "slots", "status", "ticket", "requests", "tokens", "addresses")
 
     def __init__(self, backend, requests: int, tokens: int):
         if requests < 0 or tokens < 0:
@@ -70,6 +74,7 @@ class Kv4Step:
         self.cu, self.kv_lens = new(requests + 1), new(requests)
         self.positions, self.slots = new(tokens), new(tokens)
         self.status, self.ticket = new(1), new(1)
+        self.addresses = tuple(t.data_ptr() for t in (self.cu, self.kv_lens, self.positions, self.slots, self.status, self.ticket))
 
 
 def rope_table(positions: int, rot: int, theta: float = 1e6, device: Optional[torch.device] = None) -> torch.Tensor:
