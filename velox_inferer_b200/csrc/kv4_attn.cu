@@ -46,6 +46,8 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+constexpr int DECODE_EXTRA = 1;   // tiles' worth of an item's other costs
+
 template <int D, int NT, int WARPS>
 struct DecodeCfg {
     static constexpr int ROWS = 8 * NT;            // query rows of an item
@@ -184,7 +186,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     if (tid == 0) grid_launch_dependents();
     grid_dependency_wait();
 
-    const Run run = find_run<ROWS, TILE, C::THREADS, 4>(a, G, s_red, s_found);
+    const Run run = find_run<ROWS, TILE, DECODE_EXTRA, C::THREADS, 4>(a, G, s_red, s_found);
     if ((int)blockIdx.x >= run.blocks) return;
     const float soft = score_factor(a);
     uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws);
@@ -192,7 +194,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (tid >> 5) * (C::STAGES * C::STAGE);
     int done = 0;
-    Items<ROWS, TILE> it(a, G, run);
+    Items<ROWS, TILE, DECODE_EXTRA> it(a, G, run);
     for (; it.more(); it.next(a, G)) {
         const Request& r = it.r;
         const RowRange range = it.range;
@@ -411,7 +413,13 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
                         make_float2(o[n][i][y], o[n][i][y + 2]);
             }
         const bool whole = it.whole();
-        const int c_first = whole ? 0 : it.first_block(), c_last = whole ? 0 : it.last_block();
+        int c_first = 0, c_begin = 0, count = 1;
+        if (!whole) {
+            const auto holders = it.holders();
+            c_first = holders.first;
+            c_begin = holders.begin;
+            count = holders.end - c_begin + 1;
+        }
         float* part = parts + ((long long)blockIdx.x * 2 + ((int)blockIdx.x == c_first ? 1 : 0)) * C::PART;
         __syncthreads();
         if (tid < ROWS) {   // the warps' factors, and the row's maximum and sum
@@ -457,13 +465,12 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
         if (!whole) {
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(&tickets[c_first], 1u) == (uint32_t)(c_last - c_first);
+            if (tid == 0) s_last = atomicAdd(&tickets[c_first], 1u) == (uint32_t)(count - 1);
             __syncthreads();
             if (s_last) {   // the item's last block: join the parts in token order
                 __threadfence();
                 if (tid == 0) tickets[c_first] = 0;
-                const int count = c_last - c_first + 1;
-                auto part_of = [&](int c) { return parts + ((long long)(c_first + c) * 2 + (c == 0 ? 1 : 0)) * C::PART; };
+                auto part_of = [&](int c) { return parts + ((long long)(c_begin + c) * 2 + (c_begin + c == c_first ? 1 : 0)) * C::PART; };
                 float* s_f = smem;                      // [count][ROWS]: maxima, then factors
                 float* s_l = smem + count * ROWS;       // sums
                 for (int i = tid; i < count * ROWS; i += C::THREADS) {
@@ -517,7 +524,7 @@ static int attn_sms() {
 
 constexpr int DECODE_WARPS = 8, DECODE_PER_SM = 2;
 // Query rows per kv head and request up to which the decode kernel takes a request.
-constexpr int DECODE_ROWS = 16;
+constexpr int DECODE_ROWS = 32;
 
 // [decode tickets][prefill tickets][decode parts][prefill parts]; the tickets are zero between calls
 struct WsLayout {
@@ -531,7 +538,7 @@ static WsLayout ws_layout(int head_dim) {
     auto up = [](long long x) { return (x + 255) & ~255LL; };
     w.prefill_tickets = up(4LL * w.decode_blocks);
     w.decode_parts = up(w.prefill_tickets + 8LL * w.prefill_blocks);
-    w.prefill_parts = up(w.decode_parts + (long long)w.decode_blocks * 2 * DECODE_ROWS * (head_dim + 2) * 4);
+    w.prefill_parts = up(w.decode_parts + (long long)w.decode_blocks * 2 * 16 * (head_dim + 2) * 4);
     w.bytes = w.prefill_parts + kv4_prefill_parts_bytes(w.prefill_blocks, head_dim);
     return w;
 }

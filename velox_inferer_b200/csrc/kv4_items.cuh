@@ -1,6 +1,9 @@
 // How the attention kernels cut a step: items (request, kv head, tile of query rows), laid end to
 // end in units of one tile of tokens, an equal run of units per block. The lengths live on the
-// device, so every block finds its run itself.
+// device, so every block finds its run itself. What an item costs beside its tiles (its queries, its
+// result) counts as EXTRA more units, spread evenly over it: without them a block that met many
+// short items ended long after the others (chunks of several prompts beside decoding requests: 230 us
+// against XXX us).
 #pragma once
 
 #include "common.cuh"
@@ -48,26 +51,26 @@ __device__ __forceinline__ Request request_of(const Kv4AttnArgs& a, int G, int b
 }
 
 // Units of one kv head of a request, by the whole warp (the same request in every lane).
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, int EXTRA>
 __device__ __forceinline__ long long warp_units(const Kv4AttnArgs& a, int G, int n, int kv_len, int row_tiles) {
     long long sum = 0;
-    for (int t = threadIdx.x & 31; t < row_tiles; t += 32) sum += tiles_of<TILE>(rows_range<ROWS>(a, G, n, kv_len, t));
+    for (int t = threadIdx.x & 31; t < row_tiles; t += 32) sum += EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, n, kv_len, t));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
 // The same for a request per lane: a lane counts a single row tile itself, the warp together counts the others'.
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, int EXTRA>
 __device__ __forceinline__ long long lane_units(const Kv4AttnArgs& a, int G, int b, int& row_tiles) {
     Request r{};
     if (b < a.requests) r = request_of<ROWS>(a, G, b);
     row_tiles = r.row_tiles;
-    long long units = r.row_tiles == 1 ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0;
+    long long units = r.row_tiles == 1 ? EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0;
     uint32_t many = __ballot_sync(0xffffffffu, r.row_tiles > 1);
     while (many) {
         const int src = __ffs(many) - 1;
         many &= many - 1;
-        const long long u = warp_units<ROWS, TILE>(a, G, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.kv_len, src),
+        const long long u = warp_units<ROWS, TILE, EXTRA>(a, G, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.kv_len, src),
                                                    __shfl_sync(0xffffffffu, r.row_tiles, src));
         if ((threadIdx.x & 31) == src) units = u;
     }
@@ -90,8 +93,9 @@ __device__ __forceinline__ int block_of(long long u, long long total, int n) {
     return (total < 1 << 20 ? (int)(((uint32_t)(u + 1) * (uint32_t)n + (uint32_t)total - 1) / (uint32_t)total)
                             : (int)(((u + 1) * n + total - 1) / total)) - 1;
 }
-template <int ROWS, int TILE, int THREADS, int MIN_RUN>
+template <int ROWS, int TILE, int EXTRA, int THREADS, int MIN_RUN>
 __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* red, long long* found) {
+    static_assert(MIN_RUN > EXTRA, "a run inside an item holds one tile at least");
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hkv = a.cache.kv_heads;
     Run run;
@@ -100,7 +104,7 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     int row_tiles;
     long long first = 0, mine = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
-        first = lane_units<ROWS, TILE>(a, G, base + tid, row_tiles) * hkv;
+        first = lane_units<ROWS, TILE, EXTRA>(a, G, base + tid, row_tiles) * hkv;
         mine += first + ((long long)row_tiles * hkv << ITEMS);
     }
 #pragma unroll
@@ -112,8 +116,12 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     for (int i = 0; i < WARPS; i++) run.total += red[i];
     const long long items = run.total >> ITEMS;
     run.total &= (1LL << ITEMS) - 1;
-    // Short runs of one item cost more to join than they save: MIN_RUN units per block, or an item each.
-    run.blocks = (int)min((long long)gridDim.x, max(items, (run.total + MIN_RUN - 1) / MIN_RUN));
+    // MIN_RUN units per block at least (shorter runs cost more to join than they save), but an item each. As many blocks
+    // for every item where that leaves few out or runs are short: items of one length are then cut alike, and
+    // no block has parts of two (8 requests of 4096 tokens: 20 us against 25).
+    const long long cap = min((long long)gridDim.x, max(items, run.total / MIN_RUN));
+    const long long even = items > 0 ? cap / items * items : 0;
+    run.blocks = (int)(even * 16 >= cap * 15 || run.total < 8 * cap ? max(even, min(items, cap)) : cap);
     run.request = 0;
     run.request_first = run.begin = run.end = 0;
     if ((int)blockIdx.x >= run.blocks) return run;
@@ -122,7 +130,7 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     long long before = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
         const int b = base + tid;
-        const long long v = once ? first : lane_units<ROWS, TILE>(a, G, b, row_tiles) * hkv;
+        const long long v = once ? first : lane_units<ROWS, TILE, EXTRA>(a, G, b, row_tiles) * hkv;
         long long x = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -155,8 +163,8 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     return run;
 }
 
-// Walks the items of a run. Called by whole warps.
-template <int ROWS, int TILE>
+// Walks the items of a run, those it has a tile of. Called by whole warps.
+template <int ROWS, int TILE, int EXTRA>
 struct Items {
     Request r;
     RowRange range;
@@ -174,7 +182,7 @@ struct Items {
             const int lane = threadIdx.x & 31;
             for (;; rt += 32) {
                 const int t = rt + lane;
-                const int v = t < r.row_tiles ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, t)) : 0;
+                const int v = t < r.row_tiles ? EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, t)) : 0;
                 int x = v;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -193,39 +201,60 @@ struct Items {
             }
         }
         enter(a, G);
+        if (k0 == k1) next(a, G);
     }
     __device__ __forceinline__ void load(const Kv4AttnArgs& a, int G) {
         r = request_of<ROWS>(a, G, b);
-        r.units = r.row_tiles <= 1 ? (r.row_tiles ? tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0)
-                                   : warp_units<ROWS, TILE>(a, G, r.n, r.kv_len, r.row_tiles);
+        r.units = r.row_tiles <= 1 ? (r.row_tiles ? EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0)
+                                   : warp_units<ROWS, TILE, EXTRA>(a, G, r.n, r.kv_len, r.row_tiles);
+    }
+    // Tiles before x of the item's units.
+    __device__ __forceinline__ int tile_at(long long x) const {
+        if (x <= 0) return 0;
+        if (x >= nt + EXTRA) return nt;
+        // (a 64-bit division only past 2^16 tiles)
+        return EXTRA == 0 ? (int)x : nt < 1 << 15 ? (int)((uint32_t)x * (uint32_t)nt / (uint32_t)(nt + EXTRA))
+                                                  : (int)((unsigned long long)x * nt / (unsigned)(nt + EXTRA));
     }
     __device__ __forceinline__ void enter(const Kv4AttnArgs& a, int G) {
         range = rows_range<ROWS>(a, G, r.n, r.kv_len, rt);
         nt = tiles_of<TILE>(range);
-        k0 = (int)(u - item_first);
-        k1 = (int)min((long long)nt, end - item_first);
+        k0 = tile_at(u - item_first);
+        k1 = tile_at(end - item_first);
     }
     __device__ __forceinline__ bool more() const { return u < end; }
     __device__ __forceinline__ void next(const Kv4AttnArgs& a, int G) {
-        item_first += nt;
-        u = item_first;
-        if (u >= end) return;
-        if (++rt == r.row_tiles) {
-            rt = 0;
-            if (++h == a.cache.kv_heads) {
-                h = 0;
-                do {   // (requests without rows have no units; there is one with units, since u < end)
-                    b++;
-                    load(a, G);
-                } while (r.units == 0);
+        do {
+            item_first += nt + EXTRA;
+            u = item_first;
+            if (u >= end) return;
+            if (++rt == r.row_tiles) {
+                rt = 0;
+                if (++h == a.cache.kv_heads) {
+                    h = 0;
+                    do {   // (requests without rows have no units; there is one with units, since u < end)
+                        b++;
+                        load(a, G);
+                    } while (r.units == 0);
+                }
             }
-        }
-        enter(a, G);
+            enter(a, G);
+        } while (k0 == k1);
     }
     __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nt; }
-    // First and last block that hold a part of this item.
-    __device__ __forceinline__ int first_block() const { return block_of(item_first, total, blocks); }
-    __device__ __forceinline__ int last_block() const { return block_of(item_first + nt - 1, total, blocks); }
+    // The first block whose run touches the item, and the blocks that have a tile of it (only the runs at its two ends
+    // can be too short for one).
+    struct Blocks {
+        int first, begin, end;
+    };
+    __device__ __forceinline__ Blocks holders() const {
+        Blocks x;
+        x.first = block_of(item_first, total, blocks);
+        const int last = block_of(item_first + nt + EXTRA - 1, total, blocks);
+        x.begin = x.first + (tile_at(share(total, x.first + 1, blocks) - item_first) == 0 ? 1 : 0);
+        x.end = last - (tile_at(share(total, last, blocks) - item_first) == nt ? 1 : 0);
+        return x;
+    }
 };
 
 // ---- reading the cache -------------------------------------------------------------------------

@@ -28,6 +28,7 @@ static __device__ int g_kv4_status = 0;
 enum { KV4_TIMEOUT = 7 };
 
 constexpr int PF_ROWS = 256, PF_TILE = 128, PF_THREADS = 512;
+constexpr int PF_EXTRA = 3;   // tiles' worth of an item's other costs
 
 template <int D>
 struct PrefillCfg {
@@ -121,8 +122,9 @@ struct PrefillItem {
     int tile0, hi;           // first tile, end of the tokens any row sees
     int b, h, row0, first;   // request, kv head, the request's first row, first query row (token * G + head) of the item
     int rows, n, kv_len;     // query rows of the item; the request's new and all tokens
-    int c_first, c_last;     // blocks that hold parts of it (equal: this one alone)
-    int pad[3];
+    int c_first;             // the first block whose run touches it
+    int c_begin, c_end;      // the blocks that hold parts of it (equal: this one alone)
+    int pad[2];
 };
 
 template <int D>
@@ -184,7 +186,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     }
     tc_fence_before();
     grid_dependency_wait();
-    const Run run = find_run<PF_ROWS, PF_TILE, PF_THREADS, 4>(a, G, s_red, s_found);
+    const Run run = find_run<PF_ROWS, PF_TILE, PF_EXTRA, PF_THREADS, 4>(a, G, s_red, s_found);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
@@ -192,9 +194,9 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
     // every warp that works takes the items in turn; they stay in shared memory until it gives them back
     int item_no = 0;
-    auto take = [&]() -> const PrefillItem* {
-        const int i = item_no % C::RING;
-        wait(item_full(i), (uint32_t)(item_no / C::RING) & 1u);
+    auto take = [&](int ahead = 0) -> const PrefillItem* {
+        const int no = item_no + ahead, i = no % C::RING;
+        wait(item_full(i), (uint32_t)(no / C::RING) & 1u);
         return s_items[i].k1 > 0 && !wait.given_up() ? &s_items[i] : nullptr;
     };
     auto give_back = [&]() {
@@ -218,45 +220,55 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             wait(joined(w), ph_j);
             ph_j ^= 1u;
         };
-        for (const PrefillItem* item; (item = take()) != nullptr; give_back()) {
-            const PrefillItem& it = *item;
-            const int rows = it.rows - 128 * w;   // of this half
-            if (rows <= 0) continue;
-            const int tile0 = it.tile0, qbase = it.kv_len - it.n;
-            const int rr = it.first + 128 * w + min(row, rows - 1);
-            const int tok_i = rr / G, head = it.h * G + rr % G;
-
-            // the row's Q: f16, scaled, swizzled
-            float ksc;
-            {
-                const uint16_t* p = a.q + (long long)(it.row0 + tok_i) * a.q_stride + (long long)head * D;
-                uint4 x[D / 8];
-                float amax = 0.0f;
+        // The row's Q of an item: f16, scaled, swizzled. Returns what turns its scores into powers of two. (The half's
+        // products with the Q before it are done: their scores have been read.)
+        auto load_q = [&](const PrefillItem& x) -> float {
+            const int rows = x.rows - 128 * w;
+            if (rows <= 0) return 0.0f;
+            const int rr = x.first + 128 * w + min(row, rows - 1);
+            const uint16_t* p = a.q + (long long)(x.row0 + rr / G) * a.q_stride + (long long)(x.h * G + rr % G) * D;
+            uint4 v[D / 8];
+            float amax = 0.0f;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) {
-                    x[i] = row < rows ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0);
-                    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            for (int i = 0; i < D / 8; i++) v[i] = row < rows ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(u[j] << 16)), fabsf(__uint_as_float(u[j] & 0xffff0000u))));
-                }
-                const int e = row_exponent(amax);
-                const float down = pow2(-e);
-                ksc = fmaxf(soft * pow2(e), 1e-37f);   // (a factor of 0 would turn masked scores into NaN)
+            for (int i = 0; i < D / 8; i++) {
+                const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) {
-                    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                    uint32_t y[4];
+                for (int j = 0; j < 4; j++)
+                    amax = max3(amax, fabsf(__uint_as_float(u[j] << 16)), fabsf(__uint_as_float(u[j] & 0xffff0000u)));
+            }
+            const int e = row_exponent(amax);
+            const float down = pow2(-e);
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        y[j] = pack_f16(__uint_as_float(u[j] << 16) * down, __uint_as_float(u[j] & 0xffff0000u) * down);
-                    sts16(base + C::OFF_Q + (uint32_t)(w * C::PANELS + i / 8) * C::PANEL + (uint32_t)row * 128u +
-                              (uint32_t)(((i & 7) ^ (row & 7)) << 4),
-                          make_uint4(y[0], y[1], y[2], y[3]));
-                }
+            for (int i = 0; i < D / 8; i++) {
+                const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    y[j] = pack_f16(__uint_as_float(u[j] << 16) * down, __uint_as_float(u[j] & 0xffff0000u) * down);
+                sts16(base + C::OFF_Q + (uint32_t)(w * C::PANELS + i / 8) * C::PANEL + (uint32_t)row * 128u +
+                          (uint32_t)(((i & 7) ^ (row & 7)) << 4),
+                      make_uint4(y[0], y[1], y[2], y[3]));
             }
             proxy_fence();
             mbar_arrive(q_full(w));
+            return fmaxf(soft * pow2(e), 1e-37f);   // (a factor of 0 would turn masked scores into NaN)
+        };
+        const PrefillItem* item = take();
+        float ksc_next = item != nullptr ? load_q(*item) : 0.0f;
+        for (; item != nullptr; give_back()) {
+            const PrefillItem& it = *item;
+            const float ksc = ksc_next;
+            const int rows = it.rows - 128 * w;   // of this half
+            if (rows <= 0) {
+                item = take(1);
+                if (item != nullptr) ksc_next = load_q(*item);
+                continue;
+            }
+            const int tile0 = it.tile0, qbase = it.kv_len - it.n;
+            const int rr = it.first + 128 * w + min(row, rows - 1);
+            const int tok_i = rr / G, head = it.h * G + rr % G;
 
             const int pos = qbase + tok_i;
             const int lim_hi = a.causal ? min(it.kv_len, pos + 1) : it.kv_len;
@@ -382,12 +394,16 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 mbar_arrive(p_full(w));
             }
 
+            // The next item's Q before this one's result: its first products run meanwhile.
+            item = take(1);
+            if (item != nullptr) ksc_next = load_q(*item);
+
             // ---- result ----
             wait(o_full(w), ph_o);
             ph_o ^= 1u;
             tc_fence_after();
-            const int c_first = it.c_first, c_last = it.c_last;
-            const bool whole = c_first == c_last;   // (an item split over blocks has two of them at least)
+            const int c_first = it.c_first, c_begin = it.c_begin, c_end = it.c_end;
+            const bool whole = c_begin == c_end;
             const int cta = blockIdx.x;
             uint16_t* dst = a.out + (long long)(it.row0 + tok_i) * a.out_stride + (long long)head * D;
             float* part = parts + (((long long)cta * 2 + (cta == c_first ? 1 : 0)) * 2 + w) * C::PART;
@@ -421,14 +437,14 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                 part[128 + row] = l;
                 __threadfence();
                 half_barrier();
-                if (row == 0) s_last[w] = atomicAdd(&tickets[c_first * 2 + w], 1u) == (uint32_t)(c_last - c_first);
+                if (row == 0) s_last[w] = atomicAdd(&tickets[c_first * 2 + w], 1u) == (uint32_t)(c_end - c_begin);
                 half_barrier();
                 if (s_last[w]) {   // the half's last block: join the parts in token order
                     __threadfence();
                     if (row == 0) tickets[c_first * 2 + w] = 0;
                     auto part_of = [&](int c) { return parts + (((long long)c * 2 + (c == c_first ? 1 : 0)) * 2 + w) * C::PART; };
                     float mm = NEG_BIG, ll = 0.0f;
-                    for (int c = c_first; c <= c_last; c++) {
+                    for (int c = c_begin; c <= c_end; c++) {
                         const float pm = __ldcg(part_of(c) + row), pl = __ldcg(part_of(c) + 128 + row), v = fmaxf(mm, pm);
                         ll = ll * exp2_approx(mm - v) + pl * exp2_approx(pm - v);
                         mm = v;
@@ -438,7 +454,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     for (int d = 0; d < D; d += 64) {   // sixteen loads in flight per part
                         float o[64] = {};
 #pragma unroll 1
-                        for (int c = c_first; c <= c_last; c++) {
+                        for (int c = c_begin; c <= c_end; c++) {
                             const float* q = part_of(c);
                             float4 x[16];
 #pragma unroll
@@ -646,7 +662,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             wait(drained, 0);
         } else if (warp == 13) {
             // ---------------- the items, a few ahead ----------------
-            Items<PF_ROWS, PF_TILE> items(a, G, run);
+            Items<PF_ROWS, PF_TILE, PF_EXTRA> items(a, G, run);
             for (int no = 0;; no++) {
                 const int i = no % C::RING;
                 wait(item_empty(i), ((uint32_t)(no / C::RING) & 1u) ^ 1u);
@@ -665,8 +681,12 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
                         x.rows = min(PF_ROWS, items.r.n * G - x.first);
                         x.n = items.r.n;
                         x.kv_len = items.r.kv_len;
-                        x.c_first = items.whole() ? 0 : items.first_block();
-                        x.c_last = items.whole() ? 0 : items.last_block();
+                        if (!items.whole()) {
+                            const auto holders = items.holders();
+                            x.c_first = holders.first;
+                            x.c_begin = holders.begin;
+                            x.c_end = holders.end;
+                        }
                     }
                     s_items[i] = x;
                     mbar_arrive(item_full(i));

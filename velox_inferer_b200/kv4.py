@@ -24,7 +24,7 @@ class Kv4Cache:
     magnitude is a is stored with the scale e4m3(divisor * a / 6), so magnitudes from 6 * 2**-6 / divisor up to
     2688 / divisor keep the scale's full precision (16: from 0.006 to 168)."""
 
-    __slots__ = ("storage", "page_size", "head_dim", "kv_heads", "pages", "k_divisor", "v_divisor", "struct", "ref",
+    __slots__ = ("_storage", "page_size", "head_dim", "kv_heads", "pages", "k_divisor", "v_divisor", "struct", "ref",
                  "device_index")
 
     def __init__(self, storage: torch.Tensor, page_size: int, head_dim: int, k_divisor: float = 16.0,
@@ -40,13 +40,17 @@ class Kv4Cache:
             raise Unsupported(f"4-bit cache: {pages} pages of {page_size} tokens pass 32-bit slots")
         if not (k_divisor > 0 and v_divisor > 0):
             raise ShapeError("4-bit cache: divisors are positive")
-        self.storage, self.page_size, self.head_dim = storage, page_size, head_dim
+        self._storage, self.page_size, self.head_dim = storage, page_size, head_dim
         self.pages, self.kv_heads = pages, kv_heads
         self.k_divisor, self.v_divisor = float(k_divisor), float(v_divisor)
         self.struct = _lib.Kv4CacheStruct(storage.data_ptr(), pages, page_size, kv_heads, head_dim, self.k_divisor,
                                           self.v_divisor, 0)
         self.ref = C.byref(self.struct)
         self.device_index = storage.get_device()
+
+    @property
+    def storage(self) -> torch.Tensor:
+        return self._storage
 
     @classmethod
     def alloc(cls, backend, pages: int, page_size: int, kv_heads: int, head_dim: int, k_divisor: float = 16.0,
@@ -64,17 +68,23 @@ class Kv4Step:
     """What ``Sm100Backend.kv4_plan`` writes for one step: ``cu`` [requests + 1], ``kv_lens`` [requests],
     ``positions`` and ``slots`` [tokens], ``status`` [1], all int32 on the device."""
 
-    __slots__ = ("cu", "kv_lens", "positions", "slots", "status", "ticket", "requests", "tokens", "addresses")
+    __slots__ = ("_arrays", "requests", "tokens", "addresses")
 
     def __init__(self, backend, requests: int, tokens: int):
         if requests < 0 or tokens < 0:
             raise ShapeError(f"step of {requests} requests, {tokens} tokens")
-        new = lambda n: torch.zeros(n, dtype=torch.int32, device=backend.device)  # noqa: E731
         self.requests, self.tokens = requests, tokens
-        self.cu, self.kv_lens = new(requests + 1), new(requests)
-        self.positions, self.slots = new(tokens), new(tokens)
-        self.status, self.ticket = new(1), new(1)
-        self.addresses = tuple(t.data_ptr() for t in (self.cu, self.kv_lens, self.positions, self.slots, self.status, self.ticket))
+        # ..., status, and the word the blocks of a plan count themselves with
+        self._arrays = tuple(torch.zeros(n, dtype=torch.int32, device=backend.device)
+                             for n in (requests + 1, requests, tokens, tokens, 1, 1))
+        self.addresses = tuple(t.data_ptr() for t in self._arrays)
+
+    cu = property(lambda self: self._arrays[0])
+    kv_lens = property(lambda self: self._arrays[1])
+    positions = property(lambda self: self._arrays[2])
+    slots = property(lambda self: self._arrays[3])
+    status = property(lambda self: self._arrays[4])
+    ticket = property(lambda self: self._arrays[5])
 
 
 def rope_table(positions: int, rot: int, theta: float = 1e6, device: Optional[torch.device] = None) -> torch.Tensor:
