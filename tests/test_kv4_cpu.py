@@ -173,3 +173,59 @@ def test_workspace_refusals():
     lib = _lib.lib()
     for heads, kv, D in ((0, 1, 128), (15, 2, 128), (16, 0, 128), (16, 2, 96)):
         assert lib.velox_sm100_kv4_attention_workspace(heads, kv, D) == -1
+
+
+# ---- how the attention kernels cut a step (restated from csrc/kv4_items.cuh) ---------------------------
+
+def _share(total, i, n):
+    return total * i // n
+
+
+def _block_of(u, total, n):
+    return ((u + 1) * n + total - 1) // total - 1
+
+
+def _cut(items, grid, min_run, extra):
+    """For items of `items[i]` tiles: {item: {block: (k0, k1, first, begin, end)}}."""
+    units = [nt + extra for nt in items]
+    total = sum(units)
+    cap = min(grid, max(len(items), total // min_run))
+    even = cap // len(items) * len(items)
+    n = max(even, min(len(items), cap)) if even * 16 >= cap * 15 or total < 8 * cap else cap
+    held = {i: {} for i in range(len(items))}
+    for c in range(n):
+        begin, end = _share(total, c, n), _share(total, c + 1, n)
+        assert end > begin
+        first = 0
+        for i, nt in enumerate(items):
+            stop = first + nt + extra
+            if stop > begin and first < end:
+                tile_at = lambda x: 0 if x <= 0 else nt if x >= nt + extra else x * nt // (nt + extra)  # noqa: E731,B023
+                k0, k1 = tile_at(max(begin, first) - first), tile_at(end - first)
+                f, l = _block_of(first, total, n), _block_of(stop - 1, total, n)
+                assert _share(total, f, n) <= first < _share(total, f + 1, n)
+                assert _share(total, l, n) <= stop - 1 < _share(total, l + 1, n)
+                b = f + (tile_at(_share(total, f + 1, n) - first) == 0)
+                e = l - (tile_at(_share(total, l, n) - first) == nt)
+                held[i][c] = (k0, k1, f, b, e)
+            first = stop
+    return held
+
+
+@pytest.mark.parametrize("extra", [1, 3])
+def test_every_tile_is_in_one_block_and_the_counts_agree(extra):
+    rng = np.random.default_rng(extra)
+    for _ in range(400):
+        items = [int(x) for x in rng.choice([1, 1, 2, 3, 5, 17, 64, 300], rng.choice([1, 2, 3, 8, 20, 64]))]
+        held = _cut(items, int(rng.choice([1, 2, 7, 148, 296])), 4, extra)
+        slots = set()
+        for i, nt in enumerate(items):
+            parts = {c: x for c, x in held[i].items() if x[0] < x[1]}
+            assert [t for c in sorted(parts) for t in range(*parts[c][:2])] == list(range(nt))
+            assert len({x[2:] for x in parts.values()}) == 1
+            _, _, first, begin, end = next(iter(parts.values()))
+            assert sorted(parts) == list(range(begin, end + 1))         # what the join waits for
+            for c in parts:
+                if begin != end:                                          # a parked part has a place of its own
+                    assert (c, c == first) not in slots
+                    slots.add((c, c == first))

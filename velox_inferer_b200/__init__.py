@@ -21,7 +21,7 @@ def __getattr__(name):
     if name in ("Kv4Cache", "Kv4Step", "rope_table"):
         from . import kv4
         return getattr(kv4, name)
-    if name in ("LinearStack", "StackSpec"):
+    if name in ("LinearStack", "StackAttention", "StackSpec"):
         from . import stack
         return getattr(stack, name)
     raise AttributeError(name)

@@ -8,6 +8,10 @@ Per layer, in the op order of the reference's ``Stack::forward`` (crates/velox-c
     g = silu(linear(h, gate)) * linear(h, up)                  (one fused launch)
     x += all_reduce(linear(g, down))
 
+With a ``StackAttention`` the passthrough becomes attention over a 4-bit key/value cache: the heads of q
+and k are normed and rotated, k and v written into the layer's cache, and o reads the attention's
+result.
+
 Tensor parallelism (absent from the reference, which is single-device): q/k/v/gate/up are split by
 output rows (a rank keeps rows ``[r*N/p, (r+1)*N/p)`` re-based as a smaller parent with the same
 per-tensor divisor); o/down are split along K (codes are a byte-aligned column slice, block
@@ -26,6 +30,7 @@ from typing import List, Optional
 import torch
 
 from .backend import Sm100Backend
+from .kv4 import Kv4Cache, Kv4Step, rope_table
 from .weights import ActPolicy, ActQuant, WeightFormat, WeightView, align256
 
 NV = WeightFormat.NVFP4
@@ -228,6 +233,49 @@ class LayerWeights:
     down: WeightView
 
 
+class StackAttention:
+    """The attention of a stack's layers on one rank: a 4-bit cache per layer, one page table for all of them, and the arrays
+    of a step. ``requests`` sequences are run side by side; a step gives each of them some new tokens (``plan``) and its
+    rows to ``LinearStack.forward`` in the same order. Everything runs on the device: a decode step can be captured."""
+
+    def __init__(self, backend: Sm100Backend, spec: StackSpec, requests: int, tokens: int, pages: int,
+                 page_size: int = 64, max_positions: int = 32768, theta: float = 1e6, world: int = 1):
+        s, dev = spec, backend.device
+        if s.kv_heads % world or s.heads % s.kv_heads:
+            raise ValueError(f"{s.heads} / {s.kv_heads} heads over {world} ranks")
+        self.b, self.spec, self.tokens = backend, spec, tokens
+        self.heads, self.kv_heads = s.heads // world, s.kv_heads // world
+        self.caches = [Kv4Cache.alloc(backend, pages, page_size, self.kv_heads, s.head_dim) for _ in range(s.layers)]
+        self.page_size = page_size
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.table = torch.full((requests, -(-max_positions // page_size)), -1, **i32)
+        self.free = torch.arange(pages, **i32)
+        self.taken, self.cached = torch.zeros(1, **i32), torch.zeros(requests, **i32)
+        self.step = Kv4Step(backend, requests, tokens)
+        self.rope = rope_table(max_positions, s.head_dim, theta, dev)
+        self.q_norm, self.k_norm = (torch.ones(s.head_dim, dtype=torch.float32, device=dev) for _ in range(2))
+        self.qn = torch.zeros(tokens, self.heads, s.head_dim, dtype=torch.bfloat16, device=dev)
+        self.out = torch.zeros_like(self.qn)
+        self.workspace = backend.kv4_workspace(self.heads, self.kv_heads, s.head_dim)
+        self.max_new = tokens
+
+    def plan(self, new: torch.Tensor, max_new: Optional[int] = None) -> None:
+        """Slots and pages of the next step: ``new`` [requests] int32 tokens each (device), at most ``max_new`` of them
+        (decode steps: 1). ``step.status`` tells whether the pages sufficed."""
+        self.b.kv4_plan(self.cached, new, self.table, self.free, self.taken, self.page_size, self.step)
+        self.cached.add_(new)
+        self.max_new = self.tokens if max_new is None else max_new
+
+    def run(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """The attention of one layer: projections [tokens * heads * head_dim] bf16 -> the o projection's input."""
+        b, D, st, c = self.b, self.spec.head_dim, self.step, self.caches[layer]
+        rows = lambda x, h: x[: self.tokens * h * D].view(self.tokens, h, D)  # noqa: E731
+        b.qk_norm_rope_kv4(rows(q, self.heads), rows(k, self.kv_heads), rows(v, self.kv_heads), self.q_norm, self.k_norm,
+                           self.rope, st.positions, st.slots, c, self.qn, self.spec.norm_eps)
+        b.kv4_attention(self.qn, self.out, c, self.table, st.cu, st.kv_lens, self.workspace, max_new=self.max_new)
+        return self.out
+
+
 class LinearStack:
     """The stack on one rank of a tensor-parallel group of ``world`` ranks."""
 
@@ -401,12 +449,13 @@ class LinearStack:
         b.add(self.x, part, m * h)
         return b.bf16_twin_into(self.x, self.outb, m * h)
 
-    def forward(self, xb_in: torch.Tensor, m: int) -> torch.Tensor:
+    def forward(self, xb_in: torch.Tensor, m: int, attention: Optional[StackAttention] = None) -> torch.Tensor:
         """One step over m tokens: xb_in is bf16 [m, hidden] on the device; returns the final
-        residual stream rounded to bf16 ([m, hidden], device)."""
+        residual stream rounded to bf16 ([m, hidden], device). With ``attention`` (whose step is planned and has m
+        rows) q, k and v go through it; rows behind the step's last request then carry nothing of use."""
         b, s = self.b, self.spec
         h = s.hidden
-        assert m <= self.max_tokens
+        assert m <= self.max_tokens and (attention is None or attention.tokens == m)
         launches0 = b.launch_count()
         self.x[: m * h].copy_(xb_in.reshape(-1)[: m * h])
         first = True
@@ -414,13 +463,13 @@ class LinearStack:
         # another linear emit its FP4 input from their epilogue
         q4 = self.a4 and b.linear_act(self.layers[0].q, m).kind == ActQuant.NVFP4
         emit = q4
-        for l in self.layers:
+        for li, l in enumerate(self.layers):
             # x (+= previous down partial), h = rms_norm(x)
             if q4:
                 b.add_rms_norm_q4(self.x, None, self.norm_w, None, self.hq, m, h, s.norm_eps, DIV_NORM_OUT,
                                   xb=None if first else self.pb)
                 # q feeds o directly (attention passthrough), so it is produced as o's FP4 input
-                self._qkv(l, self.hq, m, emit)
+                self._qkv(l, self.hq, m, emit and attention is None)
             else:
                 b.add_rms_norm_twin(self.x, None, self.norm_w, None, self.hb, m, h, s.norm_eps,
                                     xb=None if first else self.pb)
@@ -428,7 +477,9 @@ class LinearStack:
                 b.linear_bf16(self.hb, l.k, None, m, yb=self.kb)
                 b.linear_bf16(self.hb, l.v, None, m, yb=self.vb)
             first = False
-            if emit:
+            if attention is not None:
+                b.linear_bf16(attention.run(li, self.qb, self.kb, self.vb), l.o, None, m, yb=self.pb)
+            elif emit:
                 b.linear_q4(self.qq, DIV_O_IN, l.o, None, m, yb=self.pb)
             else:
                 b.linear_bf16(self.qb, l.o, None, m, yb=self.pb)   # attention passthrough: a = q
