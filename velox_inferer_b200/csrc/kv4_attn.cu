@@ -63,54 +63,53 @@ struct DecodeCfg {
     static constexpr int PART = ROWS * (D + 2);
 };
 
-__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
-}
+// (Offsets are immediates of the instructions: an address each in registers was a quarter of the loop's
+// instructions, and the loop is bound by their issue.)
+template <int OFF>
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0 + %2], [%1 + %2], 16;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
 }
-// The two blocks of a step into a stage, by the whole warp: 2 * 18 D bytes.
-template <int D>
+// The two blocks of a step into a stage, by the whole warp: 2 * 18 D bytes, lane by lane in 16-byte chunks.
+template <int D, int I = 0>
 __device__ __forceinline__ void copy_step(uint32_t dst, const uint8_t* p0, const uint8_t* p1, int lane) {
+    // dst, p0: at the lane's first chunk; p1: as if its block followed p0's
     constexpr int CHUNKS = 18 * D / 16, ALL = 2 * CHUNKS;   // 144 or 72 per block
-#pragma unroll
-    for (int i = 0; i < (ALL + 31) / 32; i++) {
-        const int c = lane + 32 * i;
-        const uint8_t* src = 32 * i + 31 < CHUNKS || (32 * i < CHUNKS && c < CHUNKS) ? p0 + c * 16 : p1 + (c - CHUNKS) * 16;
-        if (32 * i + 31 < ALL || c < ALL) copy16(dst + c * 16, src);
+    if constexpr (32 * I < ALL) {
+        constexpr bool first = 32 * I + 31 < CHUNKS, both = 32 * I < CHUNKS && !first;
+        const uint8_t* src = first || (both && lane < CHUNKS - 32 * I) ? p0 : p1;
+        if (32 * I + 31 < ALL || lane < ALL - 32 * I) copy16<512 * I>(dst, src);
+        copy_step<D, I + 1>(dst, p0, p1, lane);
     }
 }
 // A lane's operands of a block in shared memory.
-template <int D>
-__device__ __forceinline__ void lds_plane(uint32_t (&c)[2][D / 32], uint32_t p, int lane) {
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        if (D == 128) {
-            uint32_t v[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(p + 512 * h + lane * 16));
-            c[h][0] = v[0]; c[h][1] = v[1]; c[h][D / 32 - 2] = v[2]; c[h][D / 32 - 1] = v[3];
-        } else {
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[h][0]), "=r"(c[h][1]) : "r"(p + 256 * h + lane * 8));
-        }
+template <int D, int OFF>
+__device__ __forceinline__ void lds_plane(uint32_t (&c)[2][D / 32], uint32_t lane_piece) {
+    if constexpr (D == 128) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+                     : "=r"(c[0][0]), "=r"(c[0][1]), "=r"(c[0][2]), "=r"(c[0][3]) : "r"(lane_piece), "n"(OFF));
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+                     : "=r"(c[1][0]), "=r"(c[1][1]), "=r"(c[1][2]), "=r"(c[1][3]) : "r"(lane_piece), "n"(OFF + 512));
+    } else {
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(c[0][0]), "=r"(c[0][1]) : "r"(lane_piece), "n"(OFF));
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(c[1][0]), "=r"(c[1][1]) : "r"(lane_piece), "n"(OFF + 256));
     }
 }
-template <int D>
-__device__ __forceinline__ void lds_k(KRegs<D>& r, uint32_t blk, int lane) {
-    lds_plane<D>(r.c, blk, lane);
-    if (D == 128) {
-        r.s = lds4(blk + 16 * D + lane * 4);
+// piece: the stage plus the lane's place in a code plane; k_scale, v_scale: plus its place in a scale plane.
+template <int D, int OFF>
+__device__ __forceinline__ void lds_k(KRegs<D>& r, uint32_t piece, uint32_t k_scale) {
+    lds_plane<D, OFF>(r.c, piece);
+    if constexpr (D == 128) {
+        asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(r.s) : "r"(k_scale), "n"(OFF + 16 * D));
     } else {
         uint16_t v;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(blk + 16 * D + lane * 2));
+        asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(v) : "r"(k_scale), "n"(OFF + 16 * D));
         r.s = v;
     }
 }
-template <int D>
-__device__ __forceinline__ void lds_v(VRegs<D>& r, uint32_t blk, int lane) {
-    lds_plane<D>(r.c, blk + 8 * D, lane);
-    r.s = lds4(blk + 17 * D + (D == 128 ? lane : (lane >> 3) * 4 + (lane & 3)) * 4);
+template <int D, int OFF>
+__device__ __forceinline__ void lds_v(VRegs<D>& r, uint32_t piece, uint32_t v_scale) {
+    lds_plane<D, OFF + 8 * D>(r.c, piece);
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(r.s) : "r"(v_scale), "n"(OFF + 17 * D));
 }
 
 // S^T of one block of 16 tokens: c[n] rows g, g + 8 = tokens, columns 2t, 2t + 1 of row tile n.
@@ -193,7 +192,6 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     float* parts = reinterpret_cast<float*>(a.ws + a.decode_parts);
 
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (tid >> 5) * (C::STAGES * C::STAGE);
-    int done = 0;
     Items<ROWS, TILE, DECODE_EXTRA> it(a, G, run);
     for (; it.more(); it.next(a, G)) {
         const Request& r = it.r;
@@ -202,6 +200,17 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
         const int tile0 = range.lo / TILE;
         const int rows = min(ROWS, r.n * G - rt * ROWS);
         const int qbase = r.kv_len - r.n;
+
+        // Page ids of this warp's next sixteen steps, and of the sixteen after them: lane i holds the id of block
+        // i & 1 of step i / 2.
+        const int32_t* trow = a.table + (long long)b * a.cols;
+        const int blk_hi = (range.hi + 15) >> 4;
+        const int kb0 = tile0 * (TILE / 16) + warp * 2;   // first block of step 0
+        auto page_of = [&](int k) {
+            const int kb = kb0 + (k + (lane >> 1)) * (TILE / 16) + (lane & 1);
+            return kb < blk_hi && k + (lane >> 1) < k1 ? trow[kb >> page_shift] : -1;
+        };
+        int ids = page_of(k0), ids_next = page_of(k0 + 16);
 
         // ---- the rows' operands and limits ----
         uint32_t qf[NT][D / 16][2];
@@ -263,65 +272,58 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int i = 0; i < D / 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
 
-        // Page ids of this warp's next sixteen steps, and of the sixteen after them: lane i holds the id of block
-        // i & 1 of step i / 2.
-        const int32_t* trow = a.table + (long long)b * a.cols;
-        const int blk_hi = (range.hi + 15) >> 4;
-        const int kb0 = tile0 * (TILE / 16) + warp * 2;   // first block of step 0
-        auto page_of = [&](int k) {
-            const int kb = kb0 + (k + (lane >> 1)) * (TILE / 16) + (lane & 1);
-            return kb < blk_hi && k + (lane >> 1) < k1 ? trow[kb >> page_shift] : -1;
-        };
-        int ids = page_of(k0), ids_next = page_of(k0 + 16);
-        const uint8_t* head = a.cache.blocks + ((long long)h << page_shift) * C::BLOCK;
-        const long long page_bytes = ((long long)hkv << page_shift) * C::BLOCK;
+        const uint8_t* head = a.cache.blocks + ((long long)h << page_shift) * C::BLOCK + lane * 16;
+        const uint32_t page_bytes = ((uint32_t)hkv << page_shift) * C::BLOCK, page_mask = (1u << page_shift) - 1;
         uint32_t have = 0;        // two bits per step on its way, the oldest lowest
-        int issued = k0, slot_in = 0;
+        int issued = k0;
+        uint32_t in = ring + lane * 16;
         __syncthreads();          // (the ring is the join's memory of the item before)
-        auto issue = [&]() {
+        auto issue = [&](int ahead) {   // the step `ahead` of the one that is read next
             if (issued < k1) {
                 const int at = (issued - k0) & 15;
                 if (at == 0 && issued != k0) {
                     ids = ids_next;
                     ids_next = page_of(issued + 16);
                 }
-                const uint8_t* p[2];
-                uint32_t bits = 0;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int id = __shfl_sync(0xffffffffu, ids, at * 2 + i);
-                    const int kb = kb0 + issued * (TILE / 16) + i;
-                    const bool there = (uint32_t)id < (uint32_t)a.cache.pages;
-                    bits |= there ? 1u << i : 0u;
-                    p[i] = head + (there ? id : 0) * page_bytes + (kb & ((1 << page_shift) - 1)) * C::BLOCK;
+                const uint32_t kb = kb0 + issued * (TILE / 16);
+                uint32_t id = __shfl_sync(0xffffffffu, ids, at * 2);
+                uint32_t bits = id < (uint32_t)a.cache.pages ? 3u : 0u;
+                const uint8_t* p0 = head + (unsigned long long)(bits ? id : 0u) * page_bytes + (kb & page_mask) * C::BLOCK;
+                const uint8_t* p1 = p0;   // pages of 32 tokens and more: the step's second block follows its first
+                if (page_shift == 0) {
+                    id = __shfl_sync(0xffffffffu, ids, at * 2 + 1);
+                    const bool there = id < (uint32_t)a.cache.pages;
+                    bits = (bits & 1u) | (there ? 2u : 0u);
+                    p1 = head + (unsigned long long)(there ? id : 0u) * page_bytes - C::BLOCK;
                 }
-                have |= bits << (2 * (issued - done));
-                copy_step<D>(ring + slot_in * C::STAGE, p[0], p[1], lane);
-                slot_in = slot_in == C::STAGES - 1 ? 0 : slot_in + 1;
+                have |= bits << (2 * ahead);
+                copy_step<D>(in, p0, p1, lane);
+                in = in == ring + lane * 16 + (C::STAGES - 1) * C::STAGE ? ring + lane * 16 : in + C::STAGE;
             }
             issued++;
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        done = k0;
 #pragma unroll
-        for (int i = 0; i < C::STAGES - 1; i++) issue();
+        for (int i = 0; i < C::STAGES - 1; i++) issue(i);
 
         int slot = 0;
         for (int k = k0; k < k1; k++) {
-            issue();
+            issue(C::STAGES - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
             __syncwarp();
             const uint32_t stage = ring + slot * C::STAGE;
             slot = slot == C::STAGES - 1 ? 0 : slot + 1;
             const uint32_t there = have & 3u;
             have >>= 2;
-            done = k + 1;
+            const uint32_t piece = stage + lane * (D / 8), k_scale = stage + lane * (D / 32);
+            const uint32_t v_scale = stage + (D == 128 ? lane : (lane >> 3) * 4 + (lane & 3)) * 4;
             float c[2][NT][4];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
+            {
                 KRegs<D> kr;
-                lds_k<D>(kr, stage + i * C::BLOCK, lane);
-                scores<D, NT>(kr, qf, c[i]);
+                lds_k<D, 0>(kr, piece, k_scale);
+                scores<D, NT>(kr, qf, c[0]);
+                lds_k<D, C::BLOCK>(kr, piece, k_scale);
+                scores<D, NT>(kr, qf, c[1]);
             }
             const int tok = (tile0 + k) * TILE + warp * 32;
             if (tok < all_lo || tok + 32 > all_hi || there != 3u) {
@@ -380,11 +382,12 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
                     pf[i][n][1] = transpose8x8(pack_f16(p[2], p[3]));
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
+            {
                 VRegs<D> vr;
-                lds_v<D>(vr, stage + i * C::BLOCK, lane);
-                accumulate<D, NT>(vr, pf[i], o);
+                lds_v<D, 0>(vr, piece, v_scale);
+                accumulate<D, NT>(vr, pf[0], o);
+                lds_v<D, C::BLOCK>(vr, piece, v_scale);
+                accumulate<D, NT>(vr, pf[1], o);
             }
             __syncwarp();   // before the stage is written again
         }

@@ -175,7 +175,8 @@ struct Items {
         : u(run.begin), end(run.end), total(run.total), b(run.request), blocks(run.blocks) {
         if (u >= end) return;
         load(a, G);
-        h = (int)((u - run.request_first) / r.units);
+        const long long at = u - run.request_first;   // (64-bit divisions are slow)
+        h = at < 1LL << 31 && r.units < 1LL << 31 ? (int)((uint32_t)at / (uint32_t)r.units) : (int)(at / r.units);
         item_first = run.request_first + (long long)h * r.units;
         rt = 0;
         if (r.row_tiles > 1) {   // the row tile that holds u: 32 at a time
