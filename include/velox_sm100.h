@@ -448,10 +448,12 @@ int velox_sm100_kv4_rows(const velox_sm100_kv4_cache* cache, const int32_t* slot
  * h / (heads / kv_heads). A row that sees nothing gets zeros; rows outside every request are left as they
  * were; tokens of a page outside the cache are not seen. max_new: at least the largest number of new rows of
  * any request (requests with more are left out), which selects the kernels. Sums and softmax are f32; q is
- * taken to f16 after scaling each row by a power of two, probabilities are rounded to f16.
+ * taken to f16 after scaling each row by a power of two (|q| below 2^100), probabilities are rounded to f16.
+ * out does not overlap q. table_cols * page_size and tokens * heads / kv_heads are at most 2^30.
  * workspace: velox_sm100_kv4_attention_workspace bytes (-1 where the shape is not served), 256-byte aligned,
  * zero before its first use. The calls of one stream may share it; calls that may run at the same time, or
- * captured graphs that are replayed at the same time, need one each. */
+ * captured graphs that are replayed at the same time, need one each. After a call that gave up a wait
+ * (velox_sm100_debug_status 7) it has to be zeroed. */
 long long velox_sm100_kv4_attention_workspace(int heads, int kv_heads, int head_dim);
 int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* out, long long out_stride,
                               const velox_sm100_kv4_cache* cache, const int32_t* table, int table_cols,

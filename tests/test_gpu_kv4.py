@@ -80,6 +80,16 @@ def test_plan_many_requests(requests):
     assert used == want[5] and step.status.item() == want[6]
 
 
+def test_plan_page_ids_past_the_slots():
+    """Ids whose slots would pass 32 bits, or negative ones, in the table and in the free list: no slot."""
+    tab, step, _ = run_plan(backend(), [5, 5, 16], [1, 20, 20], 16, np.array([[-7, 0, 0], [1 << 27, 0, 0], [3, 0, 0]]), [1 << 28, (1 << 27) - 1], 0, 41, False)
+    assert np.array_equal(tab, [[-7, 0, 0], [1 << 27, 1 << 28, 0], [3, (1 << 27) - 1, -1]])
+    slots = step.slots.cpu().numpy()
+    last = ((1 << 27) - 1) * 16
+    assert np.all(slots[:21] == -1) and np.array_equal(slots[21:37], last + np.arange(16)) and np.all(slots[37:] == -1)
+    assert step.kv_lens.tolist() == [6, 25, 32] and step.status.item() == 1
+
+
 # ---- norms, rotation, store --------------------------------------------------------------------------
 
 def inputs(T, hq, hkv, D, dtype, seed, wide=False):
@@ -373,6 +383,30 @@ def test_attention_pages_outside_the_cache(new):
     out = torch.zeros(T, 8, 128, dtype=torch.bfloat16, device=DEV)
     b.kv4_attention(q, out, cache, i32(table), i32(cu), i32(lens), b.kv4_workspace(8, 2, 128), max_new=new)
     check(cache, table, cu, lens, q, out, 0, 128 ** -0.5, True, 0)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_attention_pages_shared_by_requests(new, page):
+    """A common prefix: the same page ids in several rows of the table, and twice in one."""
+    b = backend()
+    lens = [150 + new, 70 + new, 3 * page + new]
+    cache, table, cu, q, T = scene(lens, [new] * 3, 8, 2, 64, page, 12)
+    table[1, :2], table[2, 1] = table[0, :2], table[2, 0]
+    out = torch.zeros(T, 8, 64, dtype=torch.bfloat16, device=DEV)
+    b.kv4_attention(q, out, cache, i32(table), i32(cu), i32(lens), b.kv4_workspace(8, 2, 64), max_new=new)
+    check(cache, table, cu, lens, q, out, 0, 0.125, True, 0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,D", [(64, 1, 64), (33, 1, 128), (100, 2, 64), (3, 3, 128), (48, 2, 128)])
+def test_attention_group_sizes(heads, kv_heads, D):
+    """Groups of 1 to 64 query heads, with one and two new tokens."""
+    b = backend()
+    lens, new = [290, 40, 7], [1, 2, 1]
+    cache, table, cu, q, T = scene(lens, new, heads, kv_heads, D, 32, heads)
+    out = torch.zeros(T, heads, D, dtype=torch.bfloat16, device=DEV)
+    b.kv4_attention(q, out, cache, i32(table), i32(cu), i32(lens), b.kv4_workspace(heads, kv_heads, D), max_new=2)
+    check(cache, table, cu, lens, q, out, 0, D ** -0.5, True, 0)
 
 
 @pytest.mark.parametrize("new", [1, 30])

@@ -109,7 +109,8 @@ def _attention(lib, cache=None, **kw):
     (dict(window=-1), ERR_SHAPE), (dict(scale=0.0), ERR_SHAPE), (dict(scale=float("nan")), ERR_SHAPE), (dict(scale=float("inf")), ERR_SHAPE),
     (dict(q=0), ERR_SHAPE), (dict(out=0), ERR_SHAPE), (dict(q=A + 2), ERR_UNSUPPORTED), (dict(qs=2047), ERR_SHAPE), (dict(qs=2049), ERR_UNSUPPORTED),
     (dict(os=2052), ERR_UNSUPPORTED), (dict(cu=0), ERR_SHAPE), (dict(kv=0), ERR_SHAPE), (dict(table=0), ERR_SHAPE), (dict(ws=0), ERR_SHAPE),
-    (dict(ws_bytes=64), ERR_SHAPE), (dict(ws=A + 16), ERR_UNSUPPORTED)])
+    (dict(ws_bytes=64), ERR_SHAPE), (dict(ws=A + 16), ERR_UNSUPPORTED), (dict(cols=(1 << 24) + 1), ERR_UNSUPPORTED),
+    (dict(tokens=(1 << 27) + 1), ERR_UNSUPPORTED)])
 def test_attention_refusals(kw, code):
     assert _attention(_lib.lib(), **kw) == code
 

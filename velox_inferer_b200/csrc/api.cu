@@ -854,6 +854,9 @@ int velox_sm100_kv4_attention(const uint16_t* q, long long q_stride, uint16_t* o
     if (rc != 0) return rc;
     if (requests < 0 || tokens < 0 || table_cols < 0 || window < 0 || max_new < 0) return VELOX_ERR_SHAPE;
     if (!(scale > 0.0f) || scale > 1e30f) return VELOX_ERR_SHAPE;
+    // lengths and row numbers are 32-bit in the kernels
+    if ((long long)table_cols * cache->page_size > 1 << 30 || (long long)tokens * (heads / cache->kv_heads) > 1 << 30)
+        return VELOX_ERR_UNSUPPORTED;
     if (requests == 0 || tokens == 0 || max_new == 0) return 0;
     if ((rc = check_rows(q, q_stride, heads, cache->head_dim, 2)) != 0) return rc;
     if ((rc = check_rows(out, out_stride, heads, cache->head_dim, 2)) != 0) return rc;

@@ -25,6 +25,8 @@ static int kv4_sms() {
 // writes its share: the requests with index % grid == block, new pages in turn, and one slice of the token rows. A new
 // page's id is read from the free list, never back from the table, so no block waits for another;
 // only `taken` needs an order when it is updated in place: the last block to have read it writes it.
+// Bound by latency: 5 us for 64 requests, 10 us for 1000 with 35,000 rows (dependent loads, two block scans per
+// 512 requests).
 constexpr int PLAN_T = 512;
 
 __device__ __forceinline__ long long plan_scan(long long v, long long* warp_sums, long long& total) {
@@ -87,7 +89,7 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
         if (b < requests && full > cols) s_flags = 2;
         if (b < requests && b % gridDim.x == blockIdx.x) {
             cu[b] = (int32_t)tok;
-            kv_lens[b] = (int32_t)min(c + n, (have + min(need, max(0LL, n_free - at))) * P);
+            kv_lens[b] = (int32_t)min(0x7fffffffLL, min(c + n, (have + min(need, max(0LL, n_free - at))) * P));
         }
         __syncthreads();
         const int here = min(PLAN_T, requests - base);
@@ -122,7 +124,8 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
                 }
             }
             positions[t] = (int32_t)p;
-            slots[t] = id < 0 ? -1 : (int32_t)((long long)id * P + p % P);
+            const long long slot = (long long)id * P + p % P;
+            slots[t] = id < 0 || slot > 0x7fffffffLL ? -1 : (int32_t)slot;
         }
         tok0 += tok_sum;
         need0 += need_sum;
@@ -168,7 +171,8 @@ int kv4_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t*
 // the token's cosines and sines are loaded once per task. Warps walk the tasks with the grid's stride, all q tasks
 // first, and request the next task's rows before they finish this one's. With one task per warp the pass waited
 // for three memory round trips per 2 KB (2048 tokens of 64 + 8 + 8 heads, bf16: 73 us); with q, k and v rows mixed
-// in a task the warps that met the k rows (f64) every time ended last (75 us); XXX us now.
+// in a task the warps that met the k rows (f64) every time ended last (75 us); 28 us now, where issue (a good 100
+// instructions per two rows) binds: its 77 MB are 12 us.
 //   q: x / sqrt(mean(x^2) + eps) * (offset + w), rotated; f32 throughout, rounded once.
 //   k on its way into the cache: the same in f64. A 4-bit code changes by a whole step when the value
 //   before it crosses a border, so the value handed to the quantiser is the correctly rounded f32 of

@@ -15,6 +15,12 @@
 //
 // Roles of the 16 warps: 0-3 and 4-7 softmax of the two halves (also their Q rows and results), 8-11
 // conversion, 12 issues the MMAs. Tensor memory: S_0, S_1 (P over their last 64 columns), O_0, O_1.
+// What bounds it: the way of a tile through one half, scores to probabilities to product, about 3700 cycles for 2 x 1024
+// cycles of MMAs (2048 rows behind 6144 tokens, 64 / 8 heads of 128: 420 us, 1140 TFLOP/s, 69 % of cuBLAS bf16).
+// Without any exponentials it takes 395 us. Tried and slower: turns between the halves' exponentials, two score
+// buffers of 64 columns per half (477), an issuing warp per half (486), a quarter of the exponentials as polynomials
+// (448). Straight-line code in the loop is kept short: with masks in line it waited for instruction fetch (510 against 449 us).
+//
 // Work is cut over the blocks as in the decode kernel (kv4_items.cuh); halves of an item that several
 // blocks share are parked and joined in token order by the last block to arrive.
 #include "common.cuh"
