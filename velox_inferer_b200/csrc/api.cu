@@ -715,6 +715,7 @@ static int kv4_geom(const velox_sm100_kv4_cache* c, Kv4Geom& g) {
     g.blocks = c->blocks;
     g.pages = c->pages;
     g.page_size = c->page_size;
+    g.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
     g.kv_heads = c->kv_heads;
     g.head_dim = c->head_dim;
     g.k_div = c->k_divisor;

@@ -68,7 +68,7 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
     const long long used = max(0, *taken);
     const long long slice = ((long long)tokens + gridDim.x - 1) / gridDim.x;
     const long long t_begin = blockIdx.x * slice, t_end = min((long long)tokens, t_begin + slice);
-    const int P = page_size;
+    const int P = page_size, sh = __ffs(page_size) - 1;   // (a power of two; 64-bit divisions are slow)
     long long tok0 = 0, need0 = 0;   // sums over the chunks before this one
     for (int base = 0; base < requests; base += PLAN_T) {
         const int b = base + threadIdx.x;
@@ -77,7 +77,7 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
             c = max(0, cached[b]);
             n = max(0, fresh[b]);
         }
-        const long long have = (c + P - 1) / P, full = (c + n + P - 1) / P;
+        const long long have = (c + P - 1) >> sh, full = (c + n + P - 1) >> sh;
         const long long want = min(full, (long long)cols), need = max(want - have, 0LL);
         long long tok_sum, need_sum;
         const long long tok = tok0 + plan_scan(n, warp_sums, tok_sum);
@@ -101,7 +101,7 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
                 const int m = (l + r) >> 1;
                 if (s_at[m] <= at_i) l = m; else r = m;
             }
-            const long long h = ((long long)s_c[l] + P - 1) / P;
+            const long long h = ((long long)s_c[l] + P - 1) >> sh;
             table[(long long)(base + l) * cols + h + (at_i - s_at[l])] = at_i < n_free ? free_pages[at_i] : -1;
         }
         // this chunk's token rows that fall into this block's slice
@@ -113,7 +113,7 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
                 if (s_cu[m] <= t) l = m; else r = m;
             }
             const long long cc = s_c[l], p = cc + t - s_cu[l];
-            const long long pi = p / P, h = (cc + P - 1) / P;
+            const long long pi = p >> sh, h = (cc + P - 1) >> sh;
             int id = -1;
             if (pi < cols) {
                 if (pi < h) {
@@ -124,7 +124,7 @@ kv4_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ 
                 }
             }
             positions[t] = (int32_t)p;
-            const long long slot = (long long)id * P + p % P;
+            const long long slot = (long long)id * P + (p & (P - 1));
             slots[t] = id < 0 || slot > 0x7fffffffLL ? -1 : (int32_t)slot;
         }
         tok0 += tok_sum;

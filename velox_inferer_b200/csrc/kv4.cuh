@@ -24,7 +24,7 @@ namespace vx {
 struct Kv4Geom {
     uint8_t* blocks;
     long long pages;
-    int page_size, kv_heads, head_dim;
+    int page_size, page_shift, kv_heads, head_dim;   // page_size = 1 << page_shift
     float k_div, v_div;
 };
 
@@ -32,11 +32,11 @@ __host__ __device__ __forceinline__ int kv4_block_bytes(int head_dim) { return 1
 
 // Start of the block that holds `slot` (= page * page_size + offset) of head h, and the token's
 // place in it.
-__device__ __forceinline__ uint8_t* kv4_block_of(const Kv4Geom& c, long long slot, int h, int& tau) {
-    const long long page = slot / c.page_size;
-    const int off = (int)(slot - page * c.page_size);
+__device__ __forceinline__ uint8_t* kv4_block_of(const Kv4Geom& c, int slot, int h, int& tau) {
+    const int off = slot & (c.page_size - 1);
     tau = off & 15;
-    return c.blocks + ((page * c.kv_heads + h) * (c.page_size >> 4) + (off >> 4)) * kv4_block_bytes(c.head_dim);
+    const long long chunk = (long long)(slot >> c.page_shift) * c.kv_heads + h;
+    return c.blocks + ((chunk << (c.page_shift - 4)) + (off >> 4)) * kv4_block_bytes(c.head_dim);
 }
 // Offsets of a token's pieces inside its block. `byte` counts the code bytes of a row (D/2 of them).
 __device__ __forceinline__ int kv4_k_code(int D, int tau, int byte) { return tau * (D / 2) + byte; }

@@ -185,7 +185,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ int s_last;
     __shared__ float s_sum[ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = __ffs(a.cache.page_size) - 5;   // (blocks per page: a power of two)
+    const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = a.cache.page_shift - 4;   // of blocks per page
     if (tid == 0) grid_launch_dependents();
     grid_dependency_wait();
 

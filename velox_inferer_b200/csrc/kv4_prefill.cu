@@ -14,7 +14,9 @@
 // maximum is only raised, and O rescaled, when it grows by more than 2^8 (P stays below 2^14).
 //
 // Roles of the 16 warps: 0-3 and 4-7 softmax of the two halves (also their Q rows and results), 8-11
-// conversion, 12 issues the MMAs. Tensor memory: S_0, S_1 (P over their last 64 columns), O_0, O_1.
+// conversion, 12 issues the MMAs, 13 finds the items. Tensor memory: S_0, S_1 (P over their last 64 columns),
+// O_0, O_1.
+//
 // What bounds it: the way of a tile through one half, scores to probabilities to product, about 3700 cycles for 2 x 1024
 // cycles of MMAs (2048 rows behind 6144 tokens, 64 / 8 heads of 128: 420 us, 1140 TFLOP/s, 69 % of cuBLAS bf16).
 // Without any exponentials it takes 395 us. Tried and slower: turns between the halves' exponentials, two score
@@ -145,7 +147,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ int s_last[2];
     __shared__ PrefillItem s_items[C::RING];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = __ffs(a.cache.page_size) - 5;   // (blocks per page: a power of two)
+    const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = a.cache.page_shift - 4;   // of blocks per page
     const uint32_t bars = base + C::OFF_BARS;
     auto k_full = [&](int s) { return bars + 8u * s; };
     auto k_empty = [&](int s) { return bars + 16u + 8u * s; };
