@@ -171,8 +171,7 @@ int kv4_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t*
 // the token's cosines and sines are loaded once per task. Warps walk the tasks with the grid's stride, all q tasks
 // first, and request the next task's rows before they finish this one's. With one task per warp the pass waited
 // for three memory round trips per 2 KB (2048 tokens of 64 + 8 + 8 heads, bf16: 73 us); with q, k and v rows mixed
-// in a task the warps that met the k rows (f64) every time ended last (75 us); 28 us now, where issue (a good 100
-// instructions per two rows) binds: its 77 MB are 12 us.
+// in a task the warps that met the k rows (f64) every time ended last (75 us); 26 us now, where instructions bind (an issue slot in two is used): its 77 MB are 12 us.
 //   q: x / sqrt(mean(x^2) + eps) * (offset + w), rotated; f32 throughout, rounded once.
 //   k on its way into the cache: the same in f64. A 4-bit code changes by a whole step when the value
 //   before it crosses a border, so the value handed to the quantiser is the correctly rounded f32 of
@@ -253,9 +252,12 @@ __device__ __forceinline__ void norm8_f32(float (&x)[8], const float* __restrict
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float inv = rsqrtf(ss * (1.0f / D) + eps);   // (two units in the last place at most)
-    const float one = offset ? 1.0f : 0.0f;
+    if (offset) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = x[i] * inv * (one + w[i]);
+        for (int i = 0; i < 8; i++) w[i] += 1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = x[i] * inv * w[i];
 }
 
 // The same in f64. 1 / sqrt by two Newton steps from the single-precision estimate (2^-22 -> 2^-44 -> 2^-88): a
@@ -335,7 +337,8 @@ kv4_norm_rope_kernel(const __grid_constant__ Kv4RopeArgs a) {
         int pos, slot;
         unsigned tok, g0;
     };
-    // Group g of a token's k / v rows: the k and the v row of a head group follow each other.
+    // Group g of a token's k / v rows: the k and the v row of a head group follow each other. A lane's place in a group
+    // of rows is lane * 8 elements in, the next group of the same operand 256 elements on.
     auto head_of = [&](bool q, unsigned g) { return (int)(q || !a.store ? g : g >> 1) * RPG + sub; };
     auto fetch = [&](unsigned task, Task& t) {
         const bool q = task < tq;
@@ -344,22 +347,19 @@ kv4_norm_rope_kernel(const __grid_constant__ Kv4RopeArgs a) {
         t.g0 = (task - t.tok * (q ? cq : ck)) * ROWS;
         t.pos = a.positions ? a.positions[t.tok] : 0;
         t.slot = a.store ? a.slots[t.tok] : 0;
+        const int bytes = F32 ? 4 : 2, heads = q ? a.heads : a.kv_heads;
+        const bool both = !q && a.store;
+        const uint8_t* at = reinterpret_cast<const uint8_t*>(q ? a.q : a.k) +
+                            ((long long)t.tok * (q ? a.q_stride : a.k_stride) + (both ? t.g0 >> 1 : t.g0) * 256 + lane * 8) * bytes;
+        const uint8_t* at_v = at;
+        if (both) at_v = reinterpret_cast<const uint8_t*>(a.v) + ((long long)t.tok * a.v_stride + (t.g0 >> 1) * 256 + lane * 8) * bytes;
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
-            const unsigned g = t.g0 + r;
-            const bool v = !q && a.store && (g & 1);
-            const int head = head_of(q, g);
-            if (head < (q ? a.heads : a.kv_heads)) {
-                const void* p = q ? a.q : v ? a.v : a.k;
-                const long long at = (long long)t.tok * (q ? a.q_stride : v ? a.v_stride : a.k_stride) + head * D + li * 8;
-                const uint4* src = F32 ? reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + at)
-                                       : reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + at);
+            const uint8_t* src = !both ? at + r * 256 * bytes : ((ROWS == 1 ? t.g0 : r) & 1 ? at_v : at) + (r >> 1) * 256 * bytes;
+            const bool on = head_of(q, t.g0 + r) < heads;
 #pragma unroll
-                for (int i = 0; i < (F32 ? 2 : 1); i++) t.x[r][i] = src[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < (F32 ? 2 : 1); i++) t.x[r][i] = make_uint4(0, 0, 0, 0);
-            }
+            for (int i = 0; i < (F32 ? 2 : 1); i++)
+                t.x[r][i] = on ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
         }
     };
 
@@ -401,7 +401,7 @@ kv4_norm_rope_kernel(const __grid_constant__ Kv4RopeArgs a) {
         if (q || !a.store) {
             const float* weight = q ? a.q_weight : a.k_weight;
             const int heads = q ? a.heads : a.kv_heads;
-            const long long at = (long long)t.tok * (q ? a.q_out_stride : a.k_out_stride) + li * 8;
+            const long long at = (long long)t.tok * (q ? a.q_out_stride : a.k_out_stride) + t.g0 * 256 + lane * 8;
 #pragma unroll
             for (int r = 0; r < ROWS; r++) {
                 const int head = (int)(t.g0 + r) * RPG + sub;
@@ -409,7 +409,7 @@ kv4_norm_rope_kernel(const __grid_constant__ Kv4RopeArgs a) {
                 if (F32) unpack8(t.x[r][0], t.x[r][F32 ? 1 : 0], x); else unpack8(t.x[r][0], x);
                 if (weight) norm8_f32<LPR>(x, weight, a.offset, a.eps, li);
                 if (a.rope) rotate8(x, turn, a.interleaved);
-                if (head < heads) store_row8(q ? a.q_out : a.k_out, at + head * D, a.out_f32, x);
+                if (head < heads) store_row8(q ? a.q_out : a.k_out, at + r * 256, a.out_f32, x);
             }
         } else {
             const bool keep = t.slot >= 0 && t.slot < slots;
