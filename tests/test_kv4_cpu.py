@@ -230,3 +230,37 @@ def test_every_tile_is_in_one_block_and_the_counts_agree(extra):
                 if begin != end:                                          # a parked part has a place of its own
                     assert (c, c == first) not in slots
                     slots.add((c, c == first))
+
+
+def _cut_by_items(items, grid, parts):
+    """Items by themselves: {item: {block: (k0, k1, begin, end)}}, whole or in `parts` runs, several whole ones per block where
+    there are more items than blocks."""
+    held = {i: {} for i in range(len(items))}
+    total = len(items) * parts
+    blocks = min(grid, total)
+    for c in range(blocks):
+        begin, end = _share(total, c, blocks), _share(total, c + 1, blocks)
+        for i in range(begin // parts, (end - 1) // parts + 1):
+            nt, first = items[i], i * parts
+            some = min(parts, nt)
+            tile_at = lambda x: 0 if x <= 0 else nt if x >= some else x * nt // some  # noqa: E731,B023
+            k0, k1 = tile_at(max(begin, first) - first), tile_at(end - first)
+            if k0 < k1:
+                f = _block_of(first, total, blocks)
+                held[i][c] = (k0, k1, f, f + some - 1)
+    return held
+
+
+def test_items_cut_by_themselves_hold_every_tile_once():
+    rng = np.random.default_rng(10)
+    for _ in range(800):
+        items = [int(x) for x in rng.choice([1, 1, 2, 3, 5, 17, 64, 300], rng.choice([1, 2, 3, 8, 20, 64, 300]))]
+        grid = int(rng.choice([1, 2, 7, 148, 296]))
+        parts = int(rng.integers(1, max(1, grid // len(items)) + 1))
+        held = _cut_by_items(items, grid, parts)
+        for i, nt in enumerate(items):
+            assert [t for c in sorted(held[i]) for t in range(*held[i][c][:2])] == list(range(nt))
+            _, _, begin, end = next(iter(held[i].values()))
+            assert sorted(held[i]) == list(range(begin, end + 1))         # what the join waits for
+            if begin != end:                                              # a block of a shared item has no other
+                assert all(sum(c in held[k] for k in range(len(items))) == 1 for c in held[i])

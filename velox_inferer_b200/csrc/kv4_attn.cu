@@ -51,6 +51,7 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 }
 
 constexpr int DECODE_EXTRA = 1;   // tiles' worth of an item's other costs
+constexpr int DECODE_JOIN = 3;    // and of joining its parts
 
 template <int D, int NT, int WARPS>
 struct DecodeCfg {
@@ -178,25 +179,27 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 2 : 1)
 kv4_decode_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using C = DecodeCfg<D, NT, WARPS>;
     constexpr int ROWS = C::ROWS, TILE = C::TILE;
-    extern __shared__ __align__(16) float smem[];
+    // (128: copies into rows of it that straddle lines cost 8 % at long lengths)
+    extern __shared__ __align__(128) float smem[];
     float* s_o = smem;                                   // [WARPS][ROWS][STRIDE]
     float* s_m = smem + WARPS * ROWS * C::STRIDE;        // [WARPS][ROWS] max, then sum
     __shared__ long long s_red[WARPS], s_found[2];
     __shared__ int s_last;
+    __shared__ Cut s_cut;
     __shared__ float s_sum[ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = a.cache.page_shift - 4;   // of blocks per page
     if (tid == 0) grid_launch_dependents();
     grid_dependency_wait();
 
-    const Run run = find_run<ROWS, TILE, DECODE_EXTRA, C::THREADS, 4>(a, G, s_red, s_found);
+    const Run run = find_run<ROWS, TILE, DECODE_EXTRA, C::THREADS, 4, DECODE_JOIN>(a, G, s_red, s_cut, s_found);
     if ((int)blockIdx.x >= run.blocks) return;
     const float soft = score_factor(a);
     uint32_t* tickets = reinterpret_cast<uint32_t*>(a.ws);
     float* parts = reinterpret_cast<float*>(a.ws + a.decode_parts);
 
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (tid >> 5) * (C::STAGES * C::STAGE);
-    Items<ROWS, TILE, DECODE_EXTRA> it(a, G, run);
+    Items<ROWS, TILE, DECODE_EXTRA> it(a, G, run, s_cut);
     for (; it.more(); it.next(a, G)) {
         const Request& r = it.r;
         const RowRange range = it.range;

@@ -4,6 +4,8 @@
 // result) counts as EXTRA more units, spread evenly over it: without them a block that met many
 // short items ended long after the others (chunks of several prompts beside decoding requests: 230 us
 // against 180 us).
+//
+// Short steps are cut by the item instead (see find_run): an item whole, or in parts of one block each.
 #pragma once
 
 #include "common.cuh"
@@ -51,27 +53,37 @@ __device__ __forceinline__ Request request_of(const Kv4AttnArgs& a, int G, int b
 }
 
 // Units of one kv head of a request, by the whole warp (the same request in every lane).
+// `longest`, if given, is raised to the tiles of its longest item.
 template <int ROWS, int TILE, int EXTRA>
-__device__ __forceinline__ long long warp_units(const Kv4AttnArgs& a, int G, int n, int kv_len, int row_tiles) {
+__device__ __forceinline__ long long warp_units(const Kv4AttnArgs& a, int G, int n, int kv_len, int row_tiles, int* longest = nullptr) {
     long long sum = 0;
-    for (int t = threadIdx.x & 31; t < row_tiles; t += 32) sum += EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, n, kv_len, t));
+    for (int t = threadIdx.x & 31; t < row_tiles; t += 32) {
+        const int nt = tiles_of<TILE>(rows_range<ROWS>(a, G, n, kv_len, t));
+        sum += EXTRA + nt;
+        if (longest != nullptr) *longest = max(*longest, nt);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
 }
 // The same for a request per lane: a lane counts a single row tile itself, the warp together counts the others'.
 template <int ROWS, int TILE, int EXTRA>
-__device__ __forceinline__ long long lane_units(const Kv4AttnArgs& a, int G, int b, int& row_tiles) {
+__device__ __forceinline__ long long lane_units(const Kv4AttnArgs& a, int G, int b, int& row_tiles, int& longest) {
     Request r{};
     if (b < a.requests) r = request_of<ROWS>(a, G, b);
     row_tiles = r.row_tiles;
-    long long units = r.row_tiles == 1 ? EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0;
+    long long units = 0;
+    if (r.row_tiles == 1) {
+        const int nt = tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0));
+        units = EXTRA + nt;
+        longest = max(longest, nt);
+    }
     uint32_t many = __ballot_sync(0xffffffffu, r.row_tiles > 1);
     while (many) {
         const int src = __ffs(many) - 1;
         many &= many - 1;
         const long long u = warp_units<ROWS, TILE, EXTRA>(a, G, __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.kv_len, src),
-                                                   __shfl_sync(0xffffffffu, r.row_tiles, src));
+                                                   __shfl_sync(0xffffffffu, r.row_tiles, src), &longest);
         if ((threadIdx.x & 31) == src) units = u;
     }
     return units;
@@ -83,6 +95,13 @@ struct Run {
     long long total, begin, end, request_first;
     int blocks;    // blocks that have a run
     int request;
+    int parts;     // 0: equal runs of tiles; else every item counts this many units, the parts it is cut into
+};
+// What of it is needed seldom, in shared memory: the kernels' loops need the registers.
+struct Cut {
+    long long total;
+    int blocks, parts;
+    int longest[32];   // (per warp)
 };
 // total * i / n; 64-bit divisions are slow, and most totals are small
 __device__ __forceinline__ long long share(long long total, int i, int n) {
@@ -93,35 +112,64 @@ __device__ __forceinline__ int block_of(long long u, long long total, int n) {
     return (total < 1 << 20 ? (int)(((uint32_t)(u + 1) * (uint32_t)n + (uint32_t)total - 1) / (uint32_t)total)
                             : (int)(((u + 1) * n + total - 1) / total)) - 1;
 }
-template <int ROWS, int TILE, int EXTRA, int THREADS, int MIN_RUN>
-__device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* red, long long* found) {
+template <int ROWS, int TILE, int EXTRA, int THREADS, int MIN_RUN, int JOIN>
+__device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* red, Cut& cut, long long* found) {
     static_assert(MIN_RUN > EXTRA, "a run inside an item holds one tile at least");
     constexpr int WARPS = THREADS / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hkv = a.cache.kv_heads;
     Run run;
     const bool once = a.requests <= THREADS;
     constexpr int ITEMS = 40;   // items are counted above the units
-    int row_tiles;
+    int row_tiles = 0, longest = 0;
     long long first = 0, mine = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
-        first = lane_units<ROWS, TILE, EXTRA>(a, G, base + tid, row_tiles) * hkv;
+        first = lane_units<ROWS, TILE, EXTRA>(a, G, base + tid, row_tiles, longest) * hkv;
         mine += first + ((long long)row_tiles * hkv << ITEMS);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) red[warp] = mine;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) {
+        red[warp] = mine;
+        cut.longest[warp] = longest;
+    }
     __syncthreads();
     run.total = 0;
 #pragma unroll
-    for (int i = 0; i < WARPS; i++) run.total += red[i];
+    for (int i = 0; i < WARPS; i++) {
+        run.total += red[i];
+        longest = max(longest, cut.longest[i]);
+    }
     const long long items = run.total >> ITEMS;
     run.total &= (1LL << ITEMS) - 1;
-    // MIN_RUN units per block at least (shorter runs cost more to join than they save), but an item each. As many blocks
-    // for every item where that leaves few out or runs are short: items of one length are then cut alike, and
-    // no block has parts of two (8 requests of 4096 tokens: 20 us against 25).
-    const long long cap = min((long long)gridDim.x, max(items, run.total / MIN_RUN));
-    const long long even = items > 0 ? cap / items * items : 0;
-    run.blocks = (int)(even * 16 >= cap * 15 || run.total < 8 * cap ? max(even, min(items, cap)) : cap);
+    // MIN_RUN units per block at least (shorter runs cost more to join than they save), but an item each.
+    const int grid = (int)gridDim.x;
+    run.parts = 0;
+    if (run.total < 1 << 20) {   // (64-bit divisions are slow, and most totals are small)
+        const int n = (int)items, total = (int)run.total, most = max(n, total / MIN_RUN), cap = min(grid, most);
+        // Estimates in units of the block that ends last: equal runs, which have parts of two items mostly (as many blocks
+        // for every item where they are short); items cut alike, each part a block's; whole ones, several in a block
+        // where there are more than blocks. With equal runs alone a chunk of 512 tokens took 44 us (26 whole), 256 tokens
+        // behind 1792 took 50 us (42 in two parts), 24 requests that verify three tokens in a window 21 us (15 whole).
+        const int each = n > 0 ? grid / n : 0;
+        run.blocks = total < 8 * cap ? (each > 0 ? max(n, cap / n * n) : cap) : cap;
+        const int equal = n > 0 ? total / run.blocks + 2 * EXTRA + JOIN : 0;
+        const int whole = (each > 0 ? 1 : (n + grid - 1) / grid) * (longest + EXTRA);
+        const int s = min(each, longest / MIN_RUN);
+        const int alike = s > 1 ? (longest + s - 1) / s + EXTRA + JOIN : whole;
+        if (n > 0 && min(whole, alike) <= equal) {
+            run.parts = whole <= alike ? 1 : s;
+            run.total = n * run.parts;
+            run.blocks = min(grid, n * run.parts);
+        }
+    } else {
+        run.blocks = (int)min((long long)grid, max(items, run.total / MIN_RUN));
+    }
+    if (tid == 0) {
+        cut.total = run.total;
+        cut.blocks = run.blocks;
+        cut.parts = run.parts;
+    }
     run.request = 0;
     run.request_first = run.begin = run.end = 0;
     if ((int)blockIdx.x >= run.blocks) return run;
@@ -130,7 +178,8 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
     long long before = 0;
     for (int base = 0; base < a.requests; base += THREADS) {
         const int b = base + tid;
-        const long long v = once ? first : lane_units<ROWS, TILE, EXTRA>(a, G, b, row_tiles) * hkv;
+        long long v = once ? first : lane_units<ROWS, TILE, EXTRA>(a, G, b, row_tiles, longest) * hkv;
+        if (run.parts) v = (long long)row_tiles * hkv * run.parts;
         long long x = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -139,13 +188,14 @@ __device__ __forceinline__ Run find_run(const Kv4AttnArgs& a, int G, long long* 
         }
         if (!once) {
             __syncthreads();
-            if (lane == 31) red[warp] = x;
+            if (lane == 31) red[warp] = run.parts ? x / run.parts << ITEMS : x;
             __syncthreads();
         }
         long long pre = before, sum = 0;
 #pragma unroll
         for (int i = 0; i < WARPS; i++) {
-            const long long units = red[i] & ((1LL << ITEMS) - 1);   // (the first pass's words count items too)
+            // (the first pass's words count both)
+            const long long units = run.parts ? (red[i] >> ITEMS) * run.parts : red[i] & ((1LL << ITEMS) - 1);
             pre += i < warp ? units : 0;
             sum += units;
         }
@@ -168,18 +218,22 @@ template <int ROWS, int TILE, int EXTRA>
 struct Items {
     Request r;
     RowRange range;
-    long long u, end, item_first, total;
-    int b, h, rt, nt, k0, k1, blocks;
+    long long u, end, item_first;
+    int b, h, rt, nt, k0, k1;
+    const volatile Cut& cut;
 
-    __device__ __forceinline__ Items(const Kv4AttnArgs& a, int G, const Run& run)
-        : u(run.begin), end(run.end), total(run.total), b(run.request), blocks(run.blocks) {
+    __device__ __forceinline__ Items(const Kv4AttnArgs& a, int G, const Run& run, const Cut& cut_)
+        : u(run.begin), end(run.end), b(run.request), cut(cut_) {
         if (u >= end) return;
         load(a, G);
         const long long at = u - run.request_first;   // (64-bit divisions are slow)
         h = at < 1LL << 31 && r.units < 1LL << 31 ? (int)((uint32_t)at / (uint32_t)r.units) : (int)(at / r.units);
         item_first = run.request_first + (long long)h * r.units;
         rt = 0;
-        if (r.row_tiles > 1) {   // the row tile that holds u: 32 at a time
+        if (const int parts = cut.parts) {
+            rt = (int)(u - item_first) / parts;
+            item_first += (long long)rt * parts;
+        } else if (r.row_tiles > 1) {   // the row tile that holds u: 32 at a time
             const int lane = threadIdx.x & 31;
             for (;; rt += 32) {
                 const int t = rt + lane;
@@ -206,12 +260,24 @@ struct Items {
     }
     __device__ __forceinline__ void load(const Kv4AttnArgs& a, int G) {
         r = request_of<ROWS>(a, G, b);
+        if (const int parts = cut.parts) {
+            r.units = (long long)r.row_tiles * parts;
+            return;
+        }
         r.units = r.row_tiles <= 1 ? (r.row_tiles ? EXTRA + tiles_of<TILE>(rows_range<ROWS>(a, G, r.n, r.kv_len, 0)) : 0)
                                    : warp_units<ROWS, TILE, EXTRA>(a, G, r.n, r.kv_len, r.row_tiles);
     }
+    __device__ __forceinline__ int size() const {
+        const int parts = cut.parts;
+        return parts ? parts : nt + EXTRA;
+    }
     // Tiles before x of the item's units.
-    __device__ __forceinline__ int tile_at(long long x) const {
+    __device__ __forceinline__ int tile_at(long long x, int parts) const {
         if (x <= 0) return 0;
+        if (parts) {   // an item of fewer tiles has fewer parts
+            const int some = min(parts, nt);
+            return x >= some ? nt : (int)((uint32_t)x * (uint32_t)nt / (uint32_t)some);   // (parts < 2^12, tiles < 2^20)
+        }
         if (x >= nt + EXTRA) return nt;
         // (a 64-bit division only past 2^16 tiles)
         return EXTRA == 0 ? (int)x : nt < 1 << 15 ? (int)((uint32_t)x * (uint32_t)nt / (uint32_t)(nt + EXTRA))
@@ -220,13 +286,14 @@ struct Items {
     __device__ __forceinline__ void enter(const Kv4AttnArgs& a, int G) {
         range = rows_range<ROWS>(a, G, r.n, r.kv_len, rt);
         nt = tiles_of<TILE>(range);
-        k0 = tile_at(u - item_first);
-        k1 = tile_at(end - item_first);
+        const int parts = cut.parts;
+        k0 = tile_at(u - item_first, parts);
+        k1 = tile_at(end - item_first, parts);
     }
     __device__ __forceinline__ bool more() const { return u < end; }
     __device__ __forceinline__ void next(const Kv4AttnArgs& a, int G) {
         do {
-            item_first += nt + EXTRA;
+            item_first += size();
             u = item_first;
             if (u >= end) return;
             if (++rt == r.row_tiles) {
@@ -250,10 +317,17 @@ struct Items {
     };
     __device__ __forceinline__ Blocks holders() const {
         Blocks x;
+        const long long total = cut.total;
+        const int blocks = cut.blocks;
         x.first = block_of(item_first, total, blocks);
+        if (const int parts = cut.parts) {   // a unit is a block's (or the item is whole)
+            x.begin = x.first;
+            x.end = x.first + min(parts, nt) - 1;
+            return x;
+        }
         const int last = block_of(item_first + nt + EXTRA - 1, total, blocks);
-        x.begin = x.first + (tile_at(share(total, x.first + 1, blocks) - item_first) == 0 ? 1 : 0);
-        x.end = last - (tile_at(share(total, last, blocks) - item_first) == nt ? 1 : 0);
+        x.begin = x.first + (tile_at(share(total, x.first + 1, blocks) - item_first, 0) == 0 ? 1 : 0);
+        x.end = last - (tile_at(share(total, last, blocks) - item_first, 0) == nt ? 1 : 0);
         return x;
     }
 };

@@ -37,6 +37,7 @@ enum { KV4_TIMEOUT = 7 };
 
 constexpr int PF_ROWS = 256, PF_TILE = 128, PF_THREADS = 512;
 constexpr int PF_EXTRA = 3;   // tiles' worth of an item's other costs
+constexpr int PF_JOIN = 6;    // and of joining its parts
 
 template <int D>
 struct PrefillCfg {
@@ -145,6 +146,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
     __shared__ int s_last[2];
+    __shared__ Cut s_cut;
     __shared__ PrefillItem s_items[C::RING];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hkv = a.cache.kv_heads, G = a.heads / hkv, page_shift = a.cache.page_shift - 4;   // of blocks per page
@@ -194,7 +196,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
     }
     tc_fence_before();
     grid_dependency_wait();
-    const Run run = find_run<PF_ROWS, PF_TILE, PF_EXTRA, PF_THREADS, 4>(a, G, s_red, s_found);
+    const Run run = find_run<PF_ROWS, PF_TILE, PF_EXTRA, PF_THREADS, 4, PF_JOIN>(a, G, s_red, s_cut, s_found);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
@@ -670,7 +672,7 @@ kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a) {
             wait(drained, 0);
         } else if (warp == 13) {
             // ---------------- the items, a few ahead ----------------
-            Items<PF_ROWS, PF_TILE, PF_EXTRA> items(a, G, run);
+            Items<PF_ROWS, PF_TILE, PF_EXTRA> items(a, G, run, s_cut);
             for (int no = 0;; no++) {
                 const int i = no % C::RING;
                 wait(item_empty(i), ((uint32_t)(no / C::RING) & 1u) ^ 1u);
