@@ -586,3 +586,49 @@ def test_attention_long_cache_past_32_bits():
     for x, y in zip(*outs):
         assert torch.equal(x, y)
     check(small, np.array([np.arange(5)] * 2), np.array([0, 1, 21]), [320, 300], q, outs[1][0], 0, D ** -0.5, True, 0)
+
+
+def _chosen(lens, new, G, hkv, rows, tile, extra, join, grid):
+    """Which cut csrc/kv4_items.cuh takes for causal requests without a window: 0 equal runs, else parts per item."""
+    items = []
+    for length, n in zip(lens, new):
+        for t in range(-(-n * G // rows)):
+            hi = min(length, length - n + (min((t + 1) * rows, n * G) - 1) // G + 1)
+            items += [max(1, -(-hi // tile))] * hkv
+    n, total, longest = len(items), sum(items) + extra * len(items), max(items)
+    cap = min(grid, max(n, total // 4))
+    each = grid // n
+    blocks = cap if total >= 8 * cap or not each else max(n, cap // n * n)
+    equal, whole = total // blocks + 2 * extra + join, (1 if each else -(-n // grid)) * (longest + extra)
+    s = min(each, longest // 4)
+    alike = -(-longest // s) + extra + join if s > 1 else whole
+    return 0 if min(whole, alike) > equal else 1 if whole <= alike else s
+
+
+@pytest.mark.parametrize("lens,new,hq,hkv,D,want", [
+    ([3000], [256], 16, 2, 128, "parts"),                                # prefill: both halves of an item joined
+    ([2500, 70], [40, 33], 9, 3, 64, "parts"),                           # a short item beside it has fewer parts
+    ([9000] + [120] * 30, [64] + [100] * 30, 8, 2, 128, "equal"),
+    ([130] * 90, [100] * 90, 8, 2, 64, "whole"),                         # more items than blocks
+    ([20000, 300], [1, 1], 8, 2, 128, "parts"),
+    ([5000, 40, 900], [2, 3, 1], 8, 1, 64, "parts"),
+    ([40000] + [90] * 60, [1] * 61, 8, 2, 128, "equal"),
+    ([300] * 330, [1] * 330, 8, 1, 128, "whole"),
+])
+def test_attention_every_cut(lens, new, hq, hkv, D, want):
+    """Equal runs, items in parts, whole items: the results, bit for bit the same from call to call."""
+    b = backend()
+    sms, G = torch.cuda.get_device_properties(0).multi_processor_count, hq // hkv
+    if max(new) * G > 32:
+        mode = _chosen(lens, new, G, hkv, 256, 128, 3, 6, sms)
+    else:
+        mode = _chosen(lens, new, G, hkv, 8 if max(new) * G <= 8 else 16, 256, 1, 3, 2 * sms)
+    assert {0: "equal", 1: "whole"}.get(mode, "parts") == want
+    cache, table, cu, q, T = scene(lens, new, hq, hkv, D, 64, len(lens), 1)
+    out = torch.full((T, hq, D), 0.75, dtype=torch.bfloat16, device=DEV)
+    args = (cache, i32(table), i32(cu), i32(lens), b.kv4_workspace(hq, hkv, D))
+    b.kv4_attention(q, out, *args, max_new=max(new))
+    check(cache, table, cu, lens, q, out, 0.75, D ** -0.5, True, 0)
+    again = torch.full_like(out, 0.75)
+    b.kv4_attention(q, again, *args, max_new=max(new))
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16))
