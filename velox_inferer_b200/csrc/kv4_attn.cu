@@ -19,12 +19,12 @@
 // A block or page that is not there is read from the start of the cache instead (any byte is a finite
 // number) and its scores are masked.
 //
-// Work is cut by length, on the device (the lengths live there): all (request, kv head, row tile)
-// items are laid end to end in units of one tile of tokens, every block takes an equal run. A
-// block that holds part of an item parks (max, sum, O) in the workspace, the last of the item's
+// Work is cut on the device (the lengths live there): all (request, kv head, row tile) items are laid
+// end to end in units of one tile of tokens and every block takes an equal run, or, in short steps, an item or
+// a part of one (kv4_items.cuh). A block that holds part of an item parks (max, sum, O) in the workspace, the last of the item's
 // blocks to arrive joins them in token order: results do not depend on the order of arrival.
 //
-// What bounds it: issue. A block of 16 tokens (2304 bytes) takes 340 warp instructions, 196 of them the
+// What bounds it: issue. A block of 16 tokens (2304 bytes) takes 334 warp instructions, 196 of them the
 // conversions, scalings and products of its 4096 values: 64 requests of 8192 tokens stream at 4.8 TB/s (73 % of a
 // copy; the slope between 428 and 604 MB is 6.6 TB/s), the rest is 8 us from launch to first bytes and 2 to 3 us per item.
 #include "common.cuh"
