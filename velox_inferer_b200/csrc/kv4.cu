@@ -171,7 +171,8 @@ int kv4_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t*
 // the token's cosines and sines are loaded once per task. Warps walk the tasks with the grid's stride, all q tasks
 // first, and request the next task's rows before they finish this one's. With one task per warp the pass waited
 // for three memory round trips per 2 KB (2048 tokens of 64 + 8 + 8 heads, bf16: 73 us); with q, k and v rows mixed
-// in a task the warps that met the k rows (f64) every time ended last (75 us); 26 us now, where instructions bind (an issue slot in two is used): its 77 MB are 12 us.
+// in a task the warps that met the k rows (f64) every time ended last (75 us). Now 26 us, bound by instructions (more
+// than an issue slot in two is used; its 77 MB are 12 us).
 //   q: x / sqrt(mean(x^2) + eps) * (offset + w), rotated; f32 throughout, rounded once.
 //   k on its way into the cache: the same in f64. A 4-bit code changes by a whole step when the value
 //   before it crosses a border, so the value handed to the quantiser is the correctly rounded f32 of
